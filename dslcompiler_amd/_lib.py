@@ -96,6 +96,45 @@ class MemRef2D(C.Structure):
                 ("stride1", C.c_int64)]
 
 
+class BlockNormParams(C.Structure):
+    """llk_block_norm_params."""
+    _fields_ = [("y_dtype", C.c_int), ("residual_dtype", C.c_int), ("out_dtype", C.c_int),
+                ("weight_dtype", C.c_int), ("post_weight", C.c_void_p),
+                ("pre_weight", C.c_void_p), ("gate", Tensor2D), ("residual_scale", C.c_float),
+                ("eps", C.c_float), ("weight_offset", C.c_float)]
+
+
+class Tensor3D(C.Structure):
+    """llk_tensor3d."""
+    _fields_ = [("data", C.c_void_p), ("dim0", C.c_int64), ("dim1", C.c_int64),
+                ("dim2", C.c_int64), ("stride0", C.c_int64), ("stride1", C.c_int64),
+                ("stride2", C.c_int64)]
+
+
+class Kv4Cache(C.Structure):
+    """llk_kv4_cache."""
+    _fields_ = [("data", C.c_void_p), ("pages", C.c_int64), ("page_stride", C.c_int64),
+                ("heads", C.c_int64), ("page_size", C.c_int64), ("head_dim", C.c_int64)]
+
+
+class Kv4Batch(C.Structure):
+    """llk_kv4_batch."""
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int64),
+                ("lens", C.c_void_p), ("starts", C.c_void_p), ("sequences", C.c_int64),
+                ("tokens", C.c_int64), ("max_len", C.c_int64)]
+
+
+class AttentionParams(C.Structure):
+    """llk_attention_params."""
+    _fields_ = [("scale", C.c_float), ("window", C.c_int64), ("sinks", C.c_int64)]
+
+
+class AttentionPlan(C.Structure):
+    """llk_attention_plan."""
+    _fields_ = [("rows", C.c_int), ("splits", C.c_int), ("workgroups", C.c_int64),
+                ("launches", C.c_int64), ("workspace_bytes", C.c_size_t)]
+
+
 class LLKError(RuntimeError):
     """A negative llk_status, with the library's message."""
 
@@ -108,6 +147,10 @@ P = C.c_void_p
 PP = C.POINTER(C.c_void_p)
 T2 = C.POINTER(Tensor2D)
 CTX = C.POINTER(KernelContext)
+T3 = C.POINTER(Tensor3D)
+KC = C.POINTER(Kv4Cache)
+KB = C.POINTER(Kv4Batch)
+AP = C.POINTER(AttentionParams)
 KKP = C.POINTER(KernelKeyC)
 WKP = C.POINTER(WeightKeyC)
 # llk_kernel_fn: the shape of llk_swiglu_bf16
@@ -150,6 +193,12 @@ SIGNATURES = {
     "llk_gemm_bf16": (C.c_int, [T2, P, T2, C.c_int, CTX]),
     "llk_gemm_bf16_accumulate": (C.c_int, [T2, P, T2, C.c_int, CTX]),
     "llk_mlp_bf16": (C.c_int, [T2, P, P, P, T2, T2, CTX]),
+    "llk_block_norm": (C.c_int, [T2, T2, T2, T2, C.POINTER(BlockNormParams), CTX]),
+    "llk_kv4_head_bytes": (C.c_int64, [C.c_int64, C.c_int64]),
+    "llk_kv4_write": (C.c_int, [T3, T3, KC, KB, CTX]),
+    "llk_kv4_read": (C.c_int, [KC, KB, T3, T3, CTX]),
+    "llk_kv4_attention": (C.c_int, [T3, KC, KB, AP, T3, CTX]),
+    "llk_kv4_attention_describe": (C.c_int, [T3, KC, KB, AP, C.POINTER(AttentionPlan)]),
     "llk_classify_m": (C.c_int, [C.c_int64]),
     "llk_num_tiles": (C.c_int64, [C.c_int64, C.c_int64]),
     "llk_tile_size": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64]),

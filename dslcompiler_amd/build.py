@@ -47,12 +47,16 @@ HIP_SOURCES = [
     CSRC / "kernels" / "swiglu_decode.hip",
     CSRC / "kernels" / "flex_tile.hip",
     CSRC / "kernels" / "pack.hip",
+    CSRC / "kernels" / "block_norm.hip",
+    CSRC / "kernels" / "kv4_cache.hip",
+    CSRC / "kernels" / "kv4_attention.hip",
     CSRC / "llk_abi.cpp",  # host code that calls the HIP runtime
+    CSRC / "decoder_ops.cpp",
     CSRC / "kernel_fn.cpp",
     CSRC / "code_object.cpp",
 ]
 # Host sources built by hipcc (they call the HIP runtime or hold device data).
-HIP_HOST_SOURCES = {"llk_abi.cpp", "kernel_fn.cpp", "code_object.cpp"}
+HIP_HOST_SOURCES = {"llk_abi.cpp", "decoder_ops.cpp", "kernel_fn.cpp", "code_object.cpp"}
 # One code object per operation (kernels/code_object.hip with LLK_CO_OP),
 # named as code_object.cpp looks them up.
 CODE_OBJECTS = {"llk_fused_swiglu_gfx950.hsaco": 1, "llk_matmul_gfx950.hsaco": 0}

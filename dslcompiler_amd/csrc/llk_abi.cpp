@@ -18,6 +18,7 @@
 #include <string>
 #include <vector>
 
+#include "abi_support.h"
 #include "kernels/launch.h"
 #include "packed_weights.h"
 #include "runtime/kernel_key.h"
@@ -1859,6 +1860,27 @@ int llk_mlp_bf16(const llk_tensor2d* x, const llk_packed_weights* wg, const llk_
 }
 
 }  // extern "C"
+
+namespace llk {
+
+int current_gfx950(int* dev) { return current_device(dev); }
+
+int CallWorkspace::begin(int dev, size_t bytes, llk_kernel_context* ctx) {
+  Workspace* held = nullptr;
+  const int rc = get_workspace(dev, bytes, bytes, ctx, &ptr_, &held);
+  if (rc) return rc;
+  dev_ = dev;
+  held_ = held;
+  stream_ = stream_of(ctx);
+  return LLK_OK;
+}
+
+void CallWorkspace::end() {
+  release_workspace(dev_, static_cast<Workspace*>(held_), stream_);
+  held_ = nullptr;
+}
+
+}  // namespace llk
 
 namespace llk {
 

@@ -279,6 +279,134 @@ int llk_mlp_bf16(const llk_tensor2d* x, const llk_packed_weights* wg,
                  llk_tensor2d* y, llk_tensor2d* z, llk_kernel_context* ctx);
 
 /* ----------------------------------------------------------------------- */
+/* Around the MLP in a decoder block (no counterpart in the reference,      */
+/* whose lowering stops at the MLP: LLKToLinalg.cpp:621-646)                 */
+/* ----------------------------------------------------------------------- */
+
+/* Parameters of llk_block_norm.  Element types are LLK_BF16 or LLK_FP32. */
+typedef struct llk_block_norm_params {
+  int y_dtype;        /* of y and of the gate */
+  int residual_dtype; /* of residual and residual_out */
+  int out_dtype;
+  int weight_dtype;   /* of both weights */
+  const void* post_weight; /* [N] device: the norm after the block, or NULL */
+  const void* pre_weight;  /* [N] device: the norm before the next block */
+  llk_tensor2d gate;       /* [M, N] device (stride0 0: one row for all rows);
+                              data NULL: no gate */
+  float residual_scale;
+  float eps;
+  float weight_offset;     /* added to both weights (1 for weights kept as w - 1) */
+} llk_block_norm_params;
+
+/* The step between two blocks of a decoder layer, in one launch:
+ *   u = y * rsqrt(mean(y^2) + eps) * (post_weight + weight_offset), or y
+ *   residual_out = residual + residual_scale * gate * u
+ *   out = r * rsqrt(mean(r^2) + eps) * (pre_weight + weight_offset),
+ * with r the sum before its rounding to residual_dtype.  All arithmetic in
+ * fp32.  y NULL: r = residual (the norm before the first block); then
+ * post_weight and gate must be NULL and residual_out may be.  residual_out may
+ * be residual, out may be y (the same strides).  1 <= N <= 32768; rows at any
+ * alignment of their elements.  M == 0 launches nothing. */
+int llk_block_norm(const llk_tensor2d* y, const llk_tensor2d* residual,
+                   llk_tensor2d* residual_out, llk_tensor2d* out,
+                   const llk_block_norm_params* params, llk_kernel_context* ctx);
+
+/* bf16 [dim0, dim1, dim2] with unit stride2; stride0 and stride1 in elements,
+ * in either order (rows of a result must not overlap). */
+typedef struct llk_tensor3d {
+  void* data;
+  int64_t dim0, dim1, dim2;
+  int64_t stride0, stride1, stride2;
+} llk_tensor3d;
+
+/* A cache of keys and values in 4 bits, in caller-owned device memory:
+ * [pages][heads] runs of llk_kv4_head_bytes(page_size, head_dim) bytes, each
+ * page_size / 16 tiles of 16 consecutive tokens.  A tile is 17 * head_dim
+ * bytes:
+ *   key codes [head_dim / 32][16 tokens][16 bytes], value codes likewise,
+ *   key scales [head_dim / 32][16 tokens], value scales likewise.
+ * A block of 32 consecutive values of a token is a scale byte E, standing for
+ * 2^(E - 127), and 32 codes of 4 bits (value 2i in the low half of byte i, 2i +
+ * 1 in the high half): a sign bit over an index into 0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * (the element and scale types of the OCP Microscaling FP4 format).  2^(E - 127)
+ * is the smallest power of two X with the block's largest magnitude <= 7 X, 1 <=
+ * E <= 252; codes round to nearest, ties to even, beyond 6 X to 6 X.  E = 255: a
+ * block that held an infinity or a NaN, read back as NaN. */
+typedef struct llk_kv4_cache {
+  void* data; /* 16-byte aligned */
+  int64_t pages;
+  int64_t page_stride; /* bytes, a multiple of 16 */
+  int64_t heads;
+  int64_t page_size; /* tokens: a power of two, 16 to 4096 */
+  int64_t head_dim;  /* 64, 128 or 256 */
+} llk_kv4_cache;
+
+/* Bytes of one head of a page (0 for an unsupported size). */
+int64_t llk_kv4_head_bytes(int64_t page_size, int64_t head_dim);
+
+/* The sequences of a call.  Sequence s holds lens[s] positions, position p on
+ * page table[s * table_stride + p / page_size]; its last starts[s + 1] -
+ * starts[s] positions are the call's new tokens starts[s] on.  table, lens and
+ * starts are device memory and are read by the kernels, which take a position
+ * past the table or on a page outside [0, pages) as absent. */
+typedef struct llk_kv4_batch {
+  const int32_t* table; /* [sequences, table_pages] */
+  int64_t table_stride;
+  int64_t table_pages;
+  const int32_t* lens;   /* [sequences]: positions, the new tokens included */
+  const int32_t* starts; /* [sequences + 1], ascending; NULL: one new token each */
+  int64_t sequences;
+  int64_t tokens;        /* rows of the call's tensors */
+  int64_t max_len;       /* at least the largest of lens, or 0 if not known: plans
+                            the launch; any value gives right results */
+} llk_kv4_batch;
+
+/* Quantises the new tokens' keys and values, bf16 [tokens, heads, head_dim],
+ * into the cache.  Tokens without a place (outside every sequence, before
+ * position 0, absent pages) are not written.  Two tokens with one place are the
+ * caller's error. */
+int llk_kv4_write(const llk_tensor3d* k, const llk_tensor3d* v, const llk_kv4_cache* cache,
+                  const llk_kv4_batch* batch, llk_kernel_context* ctx);
+
+/* Reads the last starts[s + 1] - starts[s] positions of every sequence back as
+ * bf16 [tokens, heads, head_dim], exactly; zeros for tokens without a place. */
+int llk_kv4_read(const llk_kv4_cache* cache, const llk_kv4_batch* batch, llk_tensor3d* k,
+                 llk_tensor3d* v, llk_kernel_context* ctx);
+
+typedef struct llk_attention_params {
+  float scale;    /* of q k^T; > 0 */
+  int64_t window; /* keys a query sees up to its own; 0: all */
+  int64_t sinks;  /* with a window: first positions that stay visible */
+} llk_attention_params;
+
+/* Attention of the new tokens' queries over the cache: q and out bf16 [tokens,
+ * q_heads, head_dim], q_heads a multiple of the cache's heads (query heads h *
+ * q_heads / heads on share key head h).  The query at position p sees key j if
+ * j <= p and (window == 0 or j > p - window or j < sinks) and j's page exists;
+ * out = softmax(scale q k^T) v over those, zeros if there are none (or if every
+ * score is -infinity).  Keys and values that a query does not see never reach
+ * its result, whatever they hold.  Softmax and sums in fp32; the weights are
+ * rounded to bf16 for the product with v.  Rows of tokens outside every
+ * sequence are not written.  Results do not change from run to run.  Workspace:
+ * llk_kv4_attention_describe. */
+int llk_kv4_attention(const llk_tensor3d* q, const llk_kv4_cache* cache,
+                      const llk_kv4_batch* batch, const llk_attention_params* params,
+                      llk_tensor3d* out, llk_kernel_context* ctx);
+
+/* The launch llk_kv4_attention chooses for a call (host-only, no HIP call; data
+ * pointers are not read). */
+typedef struct llk_attention_plan {
+  int rows;               /* query rows (new tokens x query heads of a key head) to a tile */
+  int splits;             /* parts a long sequence's keys are split into at most */
+  int64_t workgroups;     /* of the main kernel */
+  int64_t launches;
+  size_t workspace_bytes; /* = ctx->scratch size the call needs */
+} llk_attention_plan;
+int llk_kv4_attention_describe(const llk_tensor3d* q, const llk_kv4_cache* cache,
+                               const llk_kv4_batch* batch, const llk_attention_params* params,
+                               llk_attention_plan* out);
+
+/* ----------------------------------------------------------------------- */
 /* Shape specialisation and schedules                                       */
 /* ----------------------------------------------------------------------- */
 
