@@ -50,6 +50,7 @@ HIP_SOURCES = [
     CSRC / "kernels" / "block_norm.hip",
     CSRC / "kernels" / "kv4_cache.hip",
     CSRC / "kernels" / "kv4_attention.hip",
+    CSRC / "kernels" / "kv4_prompt.hip",
     CSRC / "llk_abi.cpp",  # host code that calls the HIP runtime
     CSRC / "decoder_ops.cpp",
     CSRC / "kernel_fn.cpp",

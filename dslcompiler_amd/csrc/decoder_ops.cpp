@@ -178,17 +178,19 @@ AttentionPlan plan_attention(const Kv4Batch& b, int page_shift, int heads, int g
   AttentionPlan p{};
   const int64_t rows_each = b.starts ? ((int64_t)b.tokens * group + b.sequences - 1) / b.sequences
                                      : group;
-  p.rows = rows_each <= 16 ? 16 : 32;
+  p.rows = rows_each <= 16 ? 16 : rows_each <= 32 ? 32 : kKv4PromptRows;
   p.tiles = b.starts ? (int64_t)b.tokens * group / p.rows + b.sequences
                      : (int64_t)b.sequences * ((group + p.rows - 1) / p.rows);
   int64_t len = std::min<int64_t>((int64_t)b.table_pages << page_shift, kKv4MaxLength);
   if (max_len > 0) len = std::min(len, max_len);
-  int64_t steps = (len + kKv4Step - 1) / kKv4Step;
+  const int64_t step = kv4_step(p.rows);
+  int64_t steps = (len + step - 1) / step;
   if (window > 0)
-    steps = std::min<int64_t>(steps, (sinks + kKv4Step - 1) / kKv4Step +
-                                         (window + kKv4Step - 1) / kKv4Step + 2);
+    steps = std::min<int64_t>(steps, (sinks + step - 1) / step +
+                                         (window + p.rows / group + step - 1) / step + 2);
   const int64_t groups = p.tiles * heads;
-  int64_t s = std::max<int64_t>(1, (1024 + groups - 1) / groups);
+  int64_t s = p.rows == kKv4PromptRows ? std::max<int64_t>(1, 512 / groups)
+                                      : (1024 + groups - 1) / groups;
   s = std::min<int64_t>(s, std::max<int64_t>(1, steps / 8));
   p.chunk = (int)std::max<int64_t>(1, (steps + s - 1) / s);
   p.splits = (int)std::max<int64_t>(1, (steps + p.chunk - 1) / p.chunk);

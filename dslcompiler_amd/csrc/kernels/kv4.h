@@ -65,13 +65,17 @@ hipError_t llk_launch_kv4_write(const Kv4Cache& c, const Kv4Batch& b, const Kv4R
 hipError_t llk_launch_kv4_read(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& rows, int D,
                                hipStream_t s);
 
-// Attention: `rows` is the row tile (query heads of a key head times tokens).
+// Attention: `rows` is the row tile (query heads of a key head times tokens):
+// 16 or 32, whose keys a workgroup's waves divide, or kKv4PromptRows, which
+// they divide instead.
+constexpr int kKv4PromptRows = 128;
+hipError_t llk_launch_kv4_prompt(const Kv4AttentionArgs& a, int D, hipStream_t s);
 hipError_t llk_launch_kv4_attention(const Kv4AttentionArgs& a, int D, int rows, hipStream_t s);
 size_t llk_kv4_attention_part_bytes(int64_t tiles, int heads, int splits, int rows, int D);
 // Longest sequence (and window); positions and their sums fit 32 bits.
 constexpr int kKv4MaxLength = 1 << 30;
-// Keys that one step of a row tile covers.
-constexpr int kKv4Step = 32;
+// Keys that one step of a tile of `rows` rows covers.
+constexpr int kv4_step(int rows) { return rows == kKv4PromptRows ? 64 : 32; }
 
 #ifdef __HIPCC__
 namespace llk_gfx950 {

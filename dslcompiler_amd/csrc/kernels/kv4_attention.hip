@@ -15,187 +15,15 @@
 // them: P never leaves its lane.  The codes' values are exact in bf16; P is
 // rounded to it (by 2^-8 at most, as the result is) to run on the bf16 matrix
 // instructions, while scores, maxima, sums and accumulators stay in fp32.
-#include "common.h"
-#include "kv4.h"
+#include <algorithm>
+
+#include "kv4_attention.h"
 
 namespace llk_gfx950 {
 namespace {
 
-typedef short v4i16 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4i16* lds_v4i16;
-
 constexpr int kWaves = 4;  // of a workgroup, each over its own keys
-constexpr float kNegInf = -__builtin_inff();
-
-// A row tile: its sequence, the positions its rows ask from and the steps of
-// kKv4Step keys it covers: `sink` steps from key 0, then those from `low`.
-struct RowTile {
-  int s, row0, rows;     // sequence; first row of the sequence; rows in it
-  int first, token0;     // position and index of the sequence's first new token
-  int p_lo, p_hi;        // positions of the tile's first and last query
-  int sink, low, steps;  // steps over the first tokens; first other step; all steps
-};
-
-template <int R>
-__device__ __forceinline__ bool row_tile(const Kv4AttentionArgs& a, int t, RowTile* o) {
-  const Kv4Batch& b = a.batch;
-  int first = 0, next = 0, tile0 = 0;
-  if (!b.starts) {
-    const int per = (a.group + R - 1) / R;
-    o->s = t / per;
-    first = o->s;
-    next = first + 1;
-    tile0 = o->s * per;
-  } else {
-    // sequence s has the tiles from floor(starts[s] * group / R) + s on
-    auto from = [&](int s) { return (int64_t)b.starts[s] * a.group / R + s; };
-    int lo = 0, hi = b.sequences - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (from(mid) <= t) lo = mid;
-      else hi = mid - 1;
-    }
-    o->s = lo;
-    first = b.starts[lo];
-    next = b.starts[lo + 1];
-    tile0 = (int)from(lo);
-  }
-  if (o->s >= b.sequences || t < tile0 || first < 0 || next > b.tokens) return false;
-  const int64_t row0 = (int64_t)(t - tile0) * R, all = (int64_t)(next - first) * a.group;
-  if (row0 >= all) return false;
-  o->row0 = (int)row0;
-  o->rows = (int)min((int64_t)R, all - row0);
-  o->token0 = first;
-  const int len = kv4_length(a.cache, b, o->s);
-  // new tokens past the table's end see all it holds
-  o->first = max(min(b.lens[o->s], kKv4MaxLength) - (next - first), -kKv4MaxLength);
-  o->p_lo = o->first + o->row0 / a.group;
-  o->p_hi = min(o->first + (o->row0 + o->rows - 1) / a.group, len - 1);
-  o->sink = o->low = o->steps = 0;
-  if (o->p_hi < 0) return true;
-  const int end = o->p_hi / kKv4Step + 1;
-  if (a.window) {
-    o->low = max(0, o->p_lo - a.window + 1) / kKv4Step;
-    o->sink = min((a.sinks + kKv4Step - 1) / kKv4Step, min(o->low, end));
-  }
-  o->low = min(o->low, end);
-  o->steps = o->sink + end - o->low;
-  return true;
-}
-
-// Splits that a tile's steps need (the last takes what the plan's `chunk`
-// steps to a split leave over).
-__device__ __forceinline__ int used_splits(const Kv4AttentionArgs& a, int steps) {
-  return max(1, min(a.splits, (steps + a.chunk - 1) / a.chunk));
-}
-
-// Partial planes of (tile, key head, split): O [R][D], then m [R], l [R].
-template <int D, int R>
-__device__ __forceinline__ float* part_of(const Kv4AttentionArgs& a, int tile, int head, int split) {
-  return a.part + (((int64_t)tile * a.cache.heads + head) * a.splits + split) * (R * (D + 2));
-}
-
-__device__ __forceinline__ float max_over_groups(float x) {
-  // the four lanes of a query: lane, lane ^ 16, lane ^ 32, lane ^ 48
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_over_groups(float x) {
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// 8 codes (a dword) as bf16: an MFMA operand's 16 bytes.
-__device__ __forceinline__ bf16x8 decode8(uint32_t codes, float scale) {
-  const u32x4 v{
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
-  return __builtin_bit_cast(bf16x8, v);
-}
-
-// One lane's share of a 16-token tile: D / 4 keys' codes and values' codes of
-// token lane % 16 -- the contiguous D / 4 values from lane / 16 * D / 4 (D =
-// 256: from 32 (lane / 16) and 128 + 32 (lane / 16)) -- and their scales.
-template <int D>
-struct TileCodes {
-  static constexpr int kDwords = D / 32;             // of codes, 8 values each
-  static constexpr int kScales = D == 256 ? 2 : 1;   // blocks the lane has part of
-  uint32_t k[kDwords], v[kDwords];
-  uint32_t ks[kScales], vs[kScales];  // scale bytes
-  int present;                        // the tile's page exists
-
-  __device__ __forceinline__ void load(const uint8_t* tile, int lane) {
-    if constexpr (D == 64) {
-      const int block = lane >> 5, half = (lane >> 4) & 1, tok = lane & 15;
-      const int at = (block * 16 + tok) * 16 + half * 8;
-      const uint2 a = *reinterpret_cast<const uint2*>(tile + at);
-      const uint2 b = *reinterpret_cast<const uint2*>(tile + 8 * D + at);
-      k[0] = a.x, k[1] = a.y, v[0] = b.x, v[1] = b.y;
-      ks[0] = tile[16 * D + block * 16 + tok];
-      vs[0] = tile[16 * D + D / 2 + block * 16 + tok];
-    } else {
-#pragma unroll
-      for (int c = 0; c < kScales; ++c) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(tile + c * 1024 + lane * 16);
-        const u32x4 b = *reinterpret_cast<const u32x4*>(tile + 8 * D + c * 1024 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) k[4 * c + i] = a[i], v[4 * c + i] = b[i];
-        ks[c] = tile[16 * D + c * 64 + lane];
-        vs[c] = tile[16 * D + D / 2 + c * 64 + lane];
-      }
-    }
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < kDwords; ++i) k[i] = v[i] = 0;
-#pragma unroll
-    for (int i = 0; i < kScales; ++i) ks[i] = vs[i] = 0;
-  }
-  static __device__ __forceinline__ int scale_of(int dword) { return D == 256 ? dword / 4 : 0; }
-  // First of the 8 values of dword j.
-  static __device__ __forceinline__ int element(int j, int lane) {
-    return D == 256 ? (j >> 2) * 128 + (lane >> 4) * 32 + (j & 3) * 8
-                    : (lane >> 4) * (D / 4) + j * 8;
-  }
-};
-
-// V of 32 keys in LDS, as bf16: [16-key tile][D / 16][half: 8 values][16 keys]
-// of 16 bytes, the keys of the second half swapped by 8 so that the 32 lanes
-// of a half wave, which read both halves of 8 keys, meet all 64 banks.
-template <int D>
-__device__ __forceinline__ int v_chunk(int x, int d16, int half, int key) {
-  return ((x * (D / 16) + d16) * 2 + half) * 256 + (key ^ (half * 8)) * 16;
-}
-
-// Parts of a row's softmax (maximum m of the unscaled scores, sum l, 4 of the
-// unnormalised outputs) joined into one; m is the largest of theirs.
-struct Joined {
-  float m, l = 0.0f;
-  f32x4 o{0, 0, 0, 0};
-  __device__ __forceinline__ explicit Joined(float top) : m(top) {}
-  __device__ __forceinline__ void add(float pm, float pl, const f32x4& po, float scale) {
-    const float f = __builtin_amdgcn_exp2f((pm - (m == kNegInf ? 0.0f : m)) * scale);
-    l = __builtin_fmaf(f, pl, l);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(f, po[i], o[i]);
-  }
-  // Elements d..d + 3 of the tile's row r; zeros for a row that saw no key.
-  __device__ __forceinline__ void store(const Kv4AttentionArgs& a, const RowTile& rt, int head,
-                                        int r, int d) const {
-    const int row = rt.row0 + r;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* dst = a.out + (int64_t)(rt.token0 + row / a.group) * a.out_token +
-                    (int64_t)(head * a.group + row % a.group) * a.out_head + d;
-    store8_any(dst, make_uint2(f32x2_to_bf16x2_rne(o[0] * inv, o[1] * inv),
-                               f32x2_to_bf16x2_rne(o[2] * inv, o[3] * inv)));
-  }
-};
+constexpr int kStep = 32;  // keys to a step
 
 // A workgroup's 4 waves share a row tile of 16 * RT rows and one split of its
 // keys, each wave taking every fourth step of 32 keys with a running maximum
@@ -203,7 +31,7 @@ struct Joined {
 template <int D, int RT>
 __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4AttentionArgs a) {
   constexpr int R = 16 * RT, kD16 = D / 16, kJ = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves][kKv4Step * D * 2];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves][kStep * D * 2];
   __shared__ float wave_m[kWaves][R], wave_l[kWaves][R];
   using Codes = TileCodes<D>;
   const int lane = threadIdx.x & 63;
@@ -245,7 +73,7 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4Attention
   const int page_mask = (1 << a.cache.page_shift) - 1;
   const uint8_t* const base = a.cache.data + head * a.cache.head_bytes;
   const int32_t* const table = a.batch.table + rt.s * a.batch.table_stride;
-  auto key0 = [&](int step) { return (step < rt.sink ? step : step - rt.sink + rt.low) * kKv4Step; };
+  auto key0 = [&](int step) { return (step < rt.sink ? step : step - rt.sink + rt.low) * kStep; };
   auto fetch = [&](int step, Codes (&c)[2]) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -269,8 +97,8 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4Attention
     if (step + kWaves < end) fetch(step + kWaves, next);
     const int k0 = key0(step);
     // every row sees every key of the step
-    const bool whole = k0 + kKv4Step - 1 <= rt.p_lo && cur[0].present && cur[1].present &&
-                       (!a.window || k0 > rt.p_hi - a.window || k0 + kKv4Step <= a.sinks);
+    const bool whole = k0 + kStep - 1 <= rt.p_lo && cur[0].present && cur[1].present &&
+                       (!a.window || k0 > rt.p_hi - a.window || k0 + kStep <= a.sinks);
     // V to LDS.  A value of a key that some row does not see must not reach
     // that row even as 0 * NaN: positions past the tile's last read as finite
     // (a scale of 0), and NaN blocks go in as zeros and are added to the rows
@@ -320,9 +148,7 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4Attention
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = k0 + 16 * x + 4 * grp + r;
-            const bool seen = j <= pos[y] && cur[x].present &&
-                              (!a.window || j > pos[y] - a.window || j < a.sinks);
-            st[y][x][r] = seen ? st[y][x][r] : kNegInf;
+            st[y][x][r] = cur[x].present && sees(a, pos[y], j) ? st[y][x][r] : kNegInf;
           }
       }
       float top = m[y];
@@ -380,21 +206,7 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4Attention
       for (int c = 0; c < Codes::kScales; ++c) {
         if (nan[x][c] == 0) continue;
 #pragma unroll
-        for (int y = 0; y < RT; ++y) {
-          uint32_t seen = 0;  // of the 16 keys, those the lane's row sees
-          for (int i = 0; i < 16; ++i) {
-            const int j = k0 + 16 * x + i;
-            if (j <= pos[y] && (!a.window || j > pos[y] - a.window || j < a.sinks)) seen |= 1u << i;
-          }
-#pragma unroll
-          for (int d = 0; d < kD16; ++d) {
-            // lanes that hold part of the 16 values' block: those of one group
-            const int e0 = d * 16;
-            if (D == 256 && e0 / 128 != c) continue;
-            const int g = D == 256 ? e0 % 128 / 32 : e0 / (D / 4);
-            if ((uint32_t)(nan[x][c] >> (16 * g)) & seen & 0xffffu) o[y][d] += __builtin_nanf("");
-          }
-        }
+        for (int y = 0; y < RT; ++y) add_nan<D>(a, nan[x][c], c, k0 + 16 * x, pos[y], o[y]);
       }
   }
 
@@ -437,41 +249,69 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4Attention
   }
 }
 
-// Joins a tile's splits: a workgroup per (tile, key head), its threads over
-// (row, pair of d).
+// Joins the splits of one row: a workgroup per (tile, key head; row), its
+// threads over 4 of the D elements and every kGroups-th split.
 template <int D, int R>
 __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttentionArgs a) {
+  constexpr int kPlane = R * (D + 2), kChunks = D / 4, kGroups = 256 / kChunks;
+  __shared__ f32x4 other[kGroups][kChunks];
+  __shared__ float other_l[kGroups];
   const int head = blockIdx.x % a.cache.heads, tile = blockIdx.x / a.cache.heads;
+  const int r = blockIdx.y;
   RowTile rt;
-  if (!row_tile<R>(a, tile, &rt)) return;
+  if (!row_tile<R>(a, tile, &rt) || r >= rt.rows) return;
   const int used = used_splits(a, rt.steps);
   if (used <= 1) return;
   const float* const part = part_of<D, R>(a, tile, head, 0);
-  constexpr int kPlane = R * (D + 2), kChunks = D / 4;
-  for (int i = threadIdx.x; i < rt.rows * kChunks; i += 256) {
-    const int r = i / kChunks, ch = i % kChunks;
-    Joined sum(kNegInf);
-    for (int s = 0; s < used; ++s) sum.m = fmaxf(sum.m, part[s * kPlane + R * D + r]);
-    for (int s = 0; s < used; ++s) {
-      const float* p = part + s * kPlane;
-      sum.add(p[R * D + r], p[R * (D + 1) + r],
-              reinterpret_cast<const f32x4*>(p)[r * kChunks + ch], a.scale);
-    }
-    sum.store(a, rt, head, r, ch * 4);
+  const int ch = threadIdx.x % kChunks, group = threadIdx.x / kChunks;
+  Joined sum(kNegInf);
+  for (int s = threadIdx.x & 63; s < used; s += 64)
+    sum.m = fmaxf(sum.m, part[s * kPlane + R * D + r]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum.m = fmaxf(sum.m, __shfl_xor(sum.m, d));
+#pragma unroll 4
+  for (int s = group; s < used; s += kGroups) {
+    const float* p = part + s * kPlane;
+    sum.add(p[R * D + r], p[R * (D + 1) + r],
+            reinterpret_cast<const f32x4*>(p)[r * kChunks + ch], a.scale);
   }
+  other[group][ch] = sum.o;
+  if (ch == 0) other_l[group] = sum.l;
+  __syncthreads();
+  if (group) return;
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) {
+    sum.l += other_l[g];
+    sum.o += other[g][ch];
+  }
+  sum.store(a, rt, head, r, ch * 4);
+}
+
+template <int D, int R>
+hipError_t join(const Kv4AttentionArgs& args, hipStream_t s) {
+  Kv4AttentionArgs a = args;
+  void* params[] = {&a};
+  const unsigned rows = a.batch.starts ? R : std::min(R, a.group);
+  return hipLaunchKernel(reinterpret_cast<const void*>(&kv4_join_kernel<D, R>),
+                         dim3((unsigned)(a.tiles * a.cache.heads), rows), dim3(256), params, 0, s);
 }
 
 template <int D, int RT>
-hipError_t launch(const Kv4AttentionArgs& args, hipStream_t s) {
+hipError_t attend(const Kv4AttentionArgs& args, hipStream_t s) {
   Kv4AttentionArgs a = args;
   void* params[] = {&a};
-  const unsigned x = (unsigned)(a.tiles * a.cache.heads);
-  hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&kv4_attention_kernel<D, RT>),
-                                 dim3(x, (unsigned)a.splits), dim3(kWaves * 64), params, 0, s);
-  if (e == hipSuccess && a.splits > 1)
-    e = hipLaunchKernel(reinterpret_cast<const void*>(&kv4_join_kernel<D, 16 * RT>), dim3(x),
-                        dim3(256), params, 0, s);
-  return e;
+  const hipError_t e = hipLaunchKernel(
+      reinterpret_cast<const void*>(&kv4_attention_kernel<D, RT>),
+      dim3((unsigned)(a.tiles * a.cache.heads), (unsigned)a.splits), dim3(kWaves * 64), params, 0, s);
+  return e == hipSuccess && a.splits > 1 ? join<D, 16 * RT>(a, s) : e;
+}
+
+template <int D>
+hipError_t attend_rows(const Kv4AttentionArgs& a, int rows, hipStream_t s) {
+  if (rows == 16) return attend<D, 1>(a, s);
+  if (rows == 32) return attend<D, 2>(a, s);
+  const hipError_t e = llk_launch_kv4_prompt(a, D, s);
+  return e == hipSuccess && a.splits > 1 ? join<D, kKv4PromptRows>(a, s) : e;
 }
 
 }  // namespace
@@ -479,9 +319,9 @@ hipError_t launch(const Kv4AttentionArgs& args, hipStream_t s) {
 
 hipError_t llk_launch_kv4_attention(const Kv4AttentionArgs& a, int D, int rows, hipStream_t s) {
   using namespace llk_gfx950;
-  if (rows == 16)
-    return D == 64 ? launch<64, 1>(a, s) : D == 128 ? launch<128, 1>(a, s) : launch<256, 1>(a, s);
-  return D == 64 ? launch<64, 2>(a, s) : D == 128 ? launch<128, 2>(a, s) : launch<256, 2>(a, s);
+  return D == 64    ? attend_rows<64>(a, rows, s)
+         : D == 128 ? attend_rows<128>(a, rows, s)
+                    : attend_rows<256>(a, rows, s);
 }
 
 size_t llk_kv4_attention_part_bytes(int64_t tiles, int heads, int splits, int rows, int D) {

@@ -19,20 +19,53 @@ from __future__ import annotations
 
 from . import _lib
 from ._lib import LLK_BF16, LLK_FP32, check, lib
-from .ops import _check_operand, _ctx, _torch
+from .ops import _check_operand, _check_scratch, _torch
 
 _NO_GATE = _lib.Tensor2D(None, 0, 0, 0, 0)
-_TYPES = None  # torch dtype -> llk_dtype
+_get_device = _raw_stream = None  # torch's current device and its stream's handle
+_FLOATS = _BF16 = _INT32 = _UINT8 = None  # torch dtype -> llk_dtype (0 for the others)
 
 
-def _type(t, name: str) -> int:
-    """The element type of a bf16 or fp32 operand on the current device."""
-    global _TYPES
-    if _TYPES is None:
+def _begin() -> int:
+    """The current device.  (A call of these operators is a few microseconds of
+    GPU work in a decode step: the checks below take 0.2 us an operand.)"""
+    global _get_device, _raw_stream, _FLOATS, _BF16, _INT32, _UINT8
+    if _get_device is None:
         torch = _torch()
-        _TYPES = {torch.bfloat16: LLK_BF16, torch.float32: LLK_FP32}
-    _check_operand(t, name, _TYPES)
-    return _TYPES[t.dtype]
+        _FLOATS = {torch.bfloat16: LLK_BF16, torch.float32: LLK_FP32}
+        _BF16, _INT32, _UINT8 = {torch.bfloat16: LLK_BF16}, {torch.int32: 0}, {torch.uint8: 0}
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: int(torch.cuda.current_stream(d).cuda_stream))
+        if not torch.cuda.is_available():
+            return -2  # no operand is there
+        torch.cuda.init()
+        _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    return _get_device()
+
+
+def _kind(t, name: str, dev: int, kinds) -> int:
+    """kinds' entry for the type of an operand on the current device."""
+    kind = kinds.get(getattr(t, "dtype", None))
+    if kind is None or t.get_device() != dev:
+        _check_operand(t, name, kinds)  # says what is wrong
+        raise ValueError(f"{name} is not on the current device")
+    return kind
+
+
+def _context(dev: int, stream, scratch=None) -> _lib.KernelContext:
+    handle = _raw_stream(dev) if stream is None else int(stream.cuda_stream)
+    if scratch is None:
+        return _lib.KernelContext(None, 0, handle)
+    _check_scratch(scratch)
+    return _lib.KernelContext(scratch.data_ptr(), scratch.numel() * scratch.element_size(), handle)
+
+
+def _result(like, dtype):
+    """An uninitialised contiguous tensor of like's shape and device."""
+    torch = _torch()
+    if like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)
+    return torch.empty(like.shape, dtype=dtype, device=like.device)
 
 
 def _rows(t, name: str) -> _lib.Tensor2D:
@@ -61,22 +94,22 @@ def block_norm(y, residual, pre_weight, *, post_weight=None, gate=None, scale: f
     weights are [N], both bf16 or both fp32.  y None: the norm alone (r =
     residual, which is also returned unless residual_out is given).
     residual_out may be residual itself.  out_dtype defaults to bf16."""
-    torch = _torch()
-    rtype = _type(residual, "residual")
+    dev = _begin()
+    rtype = _kind(residual, "residual", dev, _FLOATS)
     rd = _rows(residual, "residual")
     n = rd.dim1
-    wtype = _type(pre_weight, "pre_weight")
+    wtype = _kind(pre_weight, "pre_weight", dev, _FLOATS)
     post = None
     if post_weight is not None:
-        if _type(post_weight, "post_weight") != wtype:
+        if _kind(post_weight, "post_weight", dev, _FLOATS) != wtype:
             raise ValueError("post_weight and pre_weight have different types")
         post = _weight(post_weight, "post_weight", n)
-    yd, ytype, gd = None, LLK_BF16, _NO_GATE
+    yd, ytype, gd, od = None, LLK_BF16, _NO_GATE, None
     if y is not None:
-        ytype = _type(y, "y")
+        ytype = _kind(y, "y", dev, _FLOATS)
         yd = _rows(y, "y")
     if gate is not None:
-        if _type(gate, "gate") != ytype or y is None:
+        if y is None or _kind(gate, "gate", dev, _FLOATS) != ytype:
             raise ValueError("gate must have y's type")
         if gate.dim() == 1:
             if gate.shape[0] > 1 and gate.stride(0) != 1:
@@ -84,21 +117,22 @@ def block_norm(y, residual, pre_weight, *, post_weight=None, gate=None, scale: f
             gd = _lib.Tensor2D(gate.data_ptr(), rd.dim0, gate.shape[0], 0, 1)
         else:
             gd = _rows(gate, "gate")
-    if residual_out is None:
-        if y is not None:
-            residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
-        od = None if y is None else _lib.Tensor2D(residual_out.data_ptr(), rd.dim0, n, n, 1)
-    else:
-        if _type(residual_out, "residual_out") != rtype:
+    if residual_out is not None:
+        if _kind(residual_out, "residual_out", dev, _FLOATS) != rtype:
             raise ValueError("residual_out must have residual's type")
         od = _rows(residual_out, "residual_out")
+    elif y is None:
+        residual_out = residual
+    else:
+        residual_out = _result(residual, residual.dtype)
+        od = _lib.Tensor2D(residual_out.data_ptr(), rd.dim0, n, n, 1)
     if out is None:
-        out = torch.empty(residual.shape, dtype=out_dtype or torch.bfloat16, device=residual.device)
-    params = _lib.BlockNormParams(ytype, rtype, _type(out, "out"), wtype, post,
+        out = _result(residual, out_dtype or _torch().bfloat16)
+    params = _lib.BlockNormParams(ytype, rtype, _kind(out, "out", dev, _FLOATS), wtype, post,
                                   _weight(pre_weight, "pre_weight", n), gd, scale, eps,
                                   weight_offset)
-    check(lib().llk_block_norm(yd, rd, od, _rows(out, "out"), params, _ctx(stream)))
-    return (residual if residual_out is None else residual_out), out
+    check(lib().llk_block_norm(yd, rd, od, _rows(out, "out"), params, _context(dev, stream)))
+    return residual_out, out
 
 
 def kv4_cache(pages: int, heads: int, page_size: int, head_dim: int, device="cuda"):
@@ -111,42 +145,43 @@ def kv4_cache(pages: int, heads: int, page_size: int, head_dim: int, device="cud
     return torch.zeros((pages, heads, n), dtype=torch.uint8, device=device)
 
 
-def _cache(cache, head_dim: int) -> _lib.Kv4Cache:
-    _check_operand(cache, "cache", (_torch().uint8,))
+def _cache(cache, head_dim: int, dev: int) -> _lib.Kv4Cache:
+    _kind(cache, "cache", dev, _UINT8)
     if cache.dim() != 3:
         raise ValueError("cache must be [pages, heads, bytes]")
     pages, heads, n = cache.shape
     step, head, one = cache.stride()
     if (n > 1 and one != 1) or (heads > 1 and head != n):
         raise ValueError("the heads of a cache page must be contiguous")
-    size, rest = divmod(n * 16, 17 * head_dim)
+    size, rest = divmod(n * 16, 17 * head_dim) if head_dim > 0 else (0, 1)
     if rest or n == 0:
         raise ValueError(f"{n} bytes to a head are no pages of head_dim {head_dim}")
     return _lib.Kv4Cache(cache.data_ptr(), pages, step, heads, size, head_dim)
 
 
-def _batch(table, lens, starts, tokens: int, max_len) -> _lib.Kv4Batch:
-    i32 = (_torch().int32,)
-    _check_operand(table, "table", i32)
-    _check_operand(lens, "lens", i32)
-    n = lens.shape[0]
-    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != n:
+def _batch(table, lens, starts, tokens: int, max_len, dev: int) -> _lib.Kv4Batch:
+    _kind(table, "table", dev, _INT32)
+    _kind(lens, "lens", dev, _INT32)
+    if table.dim() != 2 or lens.dim() != 1:
         raise ValueError("table must be [sequences, pages] and lens [sequences]")
+    n, pages = table.shape
     step, one = table.stride()
-    if (table.shape[1] > 1 and one != 1) or (n > 1 and lens.stride(0) != 1):
+    if lens.shape[0] != n:
+        raise ValueError(f"table has {n} sequences and lens {lens.shape[0]}")
+    if (pages > 1 and one != 1) or (n > 1 and lens.stride(0) != 1):
         raise ValueError("table and lens must have unit inner stride")
     first = None
     if starts is not None:
-        _check_operand(starts, "starts", i32)
+        _kind(starts, "starts", dev, _INT32)
         if starts.dim() != 1 or starts.shape[0] != n + 1 or starts.stride(0) != 1:
             raise ValueError("starts must be a contiguous vector of sequences + 1 entries")
         first = starts.data_ptr()
-    return _lib.Kv4Batch(table.data_ptr(), step, table.shape[1], lens.data_ptr(), first, n, tokens,
+    return _lib.Kv4Batch(table.data_ptr(), step, pages, lens.data_ptr(), first, n, tokens,
                          max_len or 0)
 
 
-def _rows3(t, name: str) -> _lib.Tensor3D:
-    _check_operand(t, name, (_torch().bfloat16,))
+def _rows3(t, name: str, dev: int) -> _lib.Tensor3D:
+    _kind(t, name, dev, _BF16)
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim]")
     return _lib.Tensor3D(t.data_ptr(), *t.shape, *t.stride())
@@ -155,9 +190,11 @@ def _rows3(t, name: str) -> _lib.Tensor3D:
 def kv4_write(k, v, cache, table, lens, *, starts=None, stream=None) -> None:
     """Quantises the new tokens' keys and values, bf16 [tokens, heads,
     head_dim], into the cache; tokens without a place in it are skipped."""
-    kd = _rows3(k, "k")
-    check(lib().llk_kv4_write(kd, _rows3(v, "v"), _cache(cache, kd.dim2),
-                              _batch(table, lens, starts, kd.dim0, None), _ctx(stream)))
+    dev = _begin()
+    kd = _rows3(k, "k", dev)
+    check(lib().llk_kv4_write(kd, _rows3(v, "v", dev), _cache(cache, kd.dim2, dev),
+                              _batch(table, lens, starts, kd.dim0, None, dev),
+                              _context(dev, stream)))
 
 
 def kv4_read(cache, table, lens, *, head_dim: int, starts=None, tokens: int | None = None, k=None,
@@ -165,8 +202,8 @@ def kv4_read(cache, table, lens, *, head_dim: int, starts=None, tokens: int | No
     """(k, v) of the last starts[s + 1] - starts[s] positions of every
     sequence, bf16 [tokens, heads, head_dim]; with `starts`, `tokens` gives the
     number of rows (unless k or v is given)."""
-    torch = _torch()
-    cd = _cache(cache, head_dim)
+    dev = _begin()
+    cd = _cache(cache, head_dim, dev)
     if tokens is None:
         given = k if k is not None else v
         if given is not None:
@@ -175,21 +212,24 @@ def kv4_read(cache, table, lens, *, head_dim: int, starts=None, tokens: int | No
             tokens = lens.shape[0]
         else:
             raise ValueError("kv4_read with starts needs `tokens`")
-    shape = (tokens, cd.heads, head_dim)
+    batch = _batch(table, lens, starts, tokens, None, dev)
     if k is None:
-        k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    if v is None:
-        v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    check(lib().llk_kv4_read(cd, _batch(table, lens, starts, tokens, None), _rows3(k, "k"),
-                             _rows3(v, "v"), _ctx(stream)))
+        torch = _torch()
+        k = torch.empty((tokens, cd.heads, head_dim), dtype=torch.bfloat16, device=cache.device)
+        if v is None:
+            v = torch.empty_like(k)
+    elif v is None:
+        v = _result(k, k.dtype)
+    check(lib().llk_kv4_read(cd, batch, _rows3(k, "k", dev), _rows3(v, "v", dev),
+                             _context(dev, stream)))
     return k, v
 
 
-def _attention(q, cache, table, lens, starts, scale, window, sinks, max_len):
-    qd = _rows3(q, "q")
+def _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev):
+    qd = _rows3(q, "q", dev)
     if scale is None:
         scale = qd.dim2 ** -0.5
-    return (qd, _cache(cache, qd.dim2), _batch(table, lens, starts, qd.dim0, max_len),
+    return (qd, _cache(cache, qd.dim2, dev), _batch(table, lens, starts, qd.dim0, max_len, dev),
             _lib.AttentionParams(scale, window, sinks))
 
 
@@ -204,10 +244,11 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
     p - window or j < sinks; one that sees none gives zeros.  max_len, if the
     caller knows it, is at least the longest of lens: the launch is planned by
     it (by the table's size otherwise), and any value gives right results."""
-    args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len)
+    dev = _begin()
+    args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev)
     if out is None:
-        out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
-    check(lib().llk_kv4_attention(*args, _rows3(out, "out"), _ctx(stream, scratch)))
+        out = _result(q, q.dtype)
+    check(lib().llk_kv4_attention(*args, _rows3(out, "out", dev), _context(dev, stream, scratch)))
     return out
 
 
@@ -216,6 +257,6 @@ def describe_kv4_attention(q, cache, table, lens, *, starts=None, scale: float |
     """The launch kv4_attention chooses for these arguments."""
     p = _lib.AttentionPlan()
     check(lib().llk_kv4_attention_describe(
-        *_attention(q, cache, table, lens, starts, scale, window, sinks, max_len), p))
+        *_attention(q, cache, table, lens, starts, scale, window, sinks, max_len, _begin()), p))
     return {"rows": p.rows, "splits": p.splits, "workgroups": p.workgroups,
             "launches": p.launches, "workspace_bytes": p.workspace_bytes}
