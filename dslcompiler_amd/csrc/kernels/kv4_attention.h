@@ -96,6 +96,20 @@ __device__ __forceinline__ float sum_over_groups(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The reference m of a row's exponentials is its largest score so far, but
+// follows it only once it has grown by a factor of 2^8 of the weights: until then
+// they are at most 2^8, at no loss (the sums are fp32 and bf16 keeps its 8 bits),
+// and the accumulators need no rescaling, which 16 rows' maxima would ask for
+// at nearly every step.  top: the largest of the lane's scores and m.
+__device__ __forceinline__ bool outgrown(const Kv4AttentionArgs& a, float top, float m) {
+  return (top - m) * a.scale > 8.0f;  // m -inf: once there is a score
+}
+// What l and the accumulators are multiplied by when m becomes top.  Of a row
+// without a score yet m is -inf, and they are 0.
+__device__ __forceinline__ float rescale(const Kv4AttentionArgs& a, float top, float m) {
+  return __builtin_amdgcn_exp2f((m - (top == kNegInf ? 0.0f : top)) * a.scale);
+}
+
 // 8 codes (a dword) as bf16: an MFMA operand's 16 bytes.
 __device__ __forceinline__ bf16x8 decode8(uint32_t codes, float scale) {
   const u32x4 v{

@@ -156,10 +156,9 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_attention_kernel(Kv4Attention
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, st[y][x][r]);
-      top = max_over_groups(top);
-      if (__any(top > m[y])) {
-        // of a row that has seen no key yet m is -inf, and l and o are 0
-        const float alpha = __builtin_amdgcn_exp2f((m[y] - (top == kNegInf ? 0.0f : top)) * a.scale);
+      if (__any(outgrown(a, top, m[y]))) {
+        top = max_over_groups(top);
+        const float alpha = rescale(a, top, m[y]);
         m[y] = top;
         l[y] *= alpha;
 #pragma unroll

@@ -15,13 +15,17 @@ constexpr int kWaves = 4, kRT = 2, kRows = kKv4PromptRows, kTiles = 4;
 constexpr int kStep = 16 * kTiles;
 static_assert(kRows == kWaves * kRT * 16 && kStep == kv4_step(kRows), "row tile");
 
+constexpr uint8_t kAbsent = 1, kNan = 2;
+constexpr uint32_t kEveryTile = 0x01010101u;  // times a flag: that flag of every tile
+
 template <int D>
 struct PromptLds {
   uint8_t k[2][kStep * D * 2];  // [16-key tile][D / 32][64 lanes] of 16 bytes: A operands
   uint8_t v[2][kStep * D * 2];  // v_chunk
-  // of each 16-key tile: its page exists; lanes that hold part of a NaN block
+  // of each 16-key tile: lanes that hold part of a NaN block, and what a step
+  // looks at first, kAbsent (its page does not exist) and kNan
   uint64_t nan[2][kTiles][TileCodes<D>::kScales];
-  int present[2][kTiles];
+  uint8_t flags[2][kTiles];
 };
 
 template <int D>
@@ -34,8 +38,10 @@ __global__ void __launch_bounds__(kWaves * 64)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.y;
   const int head = blockIdx.x % a.cache.heads;
-  // the last tiles, of the most keys, first
-  const int tile = a.tiles - 1 - blockIdx.x / a.cache.heads;
+  // the last tiles, of the most keys, first; then the others from the first on,
+  // so that the two workgroups a CU gets in one round have much and little to do
+  const int nth = blockIdx.x / a.cache.heads;
+  const int tile = 2 * nth < a.tiles ? a.tiles - 1 - nth : nth - (a.tiles + 1) / 2;
   RowTile rt;
   if (!row_tile<kRows>(a, tile, &rt)) return;
   const int used = used_splits(a, rt.steps);
@@ -108,9 +114,10 @@ __global__ void __launch_bounds__(kWaves * 64)
           decode8(c.v[j], vs[Codes::scale_of(j)]);
     }
     if (lane == 0) {
-      lds.present[buf][wave] = c.present;
+      uint64_t any = 0;
 #pragma unroll
-      for (int i = 0; i < Codes::kScales; ++i) lds.nan[buf][wave][i] = nan[i];
+      for (int i = 0; i < Codes::kScales; ++i) any |= lds.nan[buf][wave][i] = nan[i];
+      lds.flags[buf][wave] = (c.present ? 0 : kAbsent) | (any ? kNan : 0);
     }
   };
 
@@ -128,30 +135,30 @@ __global__ void __launch_bounds__(kWaves * 64)
     const bool any = k0 <= w_hi &&
                      (!a.window || k0 + kStep - 1 > w_lo - a.window || k0 < a.sinks);
     if (any) {
-      bool present = true;
-      uint64_t nan = 0;
-#pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        present &= lds.present[buf][x] != 0;
-#pragma unroll
-        for (int c = 0; c < Codes::kScales; ++c) nan |= lds.nan[buf][x][c];
-      }
+      const uint32_t flags = __builtin_amdgcn_readfirstlane(
+          *reinterpret_cast<const uint32_t*>(lds.flags[buf]));
       // every row sees every key
-      const bool whole = k0 + kStep - 1 <= w_lo && present &&
+      const bool whole = k0 + kStep - 1 <= w_lo && !(flags & kAbsent * kEveryTile) &&
                          (!a.window || k0 > w_hi - a.window || k0 + kStep <= a.sinks);
       f32x4 st[kRT][kTiles];
+      bf16x8 k[2][kJ];  // of this tile, and of the next, on its way
+      auto read_k = [&](int x) {
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+          k[x & 1][j] =
+              *reinterpret_cast<const bf16x8*>(lds.k[buf] + ((x * kJ + j) * 64 + lane) * 16);
+      };
+      read_k(0);
 #pragma unroll
       for (int x = 0; x < kTiles; ++x) {
+        if (x + 1 < kTiles) read_k(x + 1);
 #pragma unroll
         for (int y = 0; y < kRT; ++y) st[y][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) {
-          const bf16x8 k =
-              *reinterpret_cast<const bf16x8*>(lds.k[buf] + ((x * kJ + j) * 64 + lane) * 16);
+        for (int j = 0; j < kJ; ++j)
 #pragma unroll
           for (int y = 0; y < kRT; ++y)
-            st[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[y][j], st[y][x], 0, 0, 0);
-        }
+            st[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[x & 1][j], q[y][j], st[y][x], 0, 0, 0);
       }
       bf16x8 p[kRT][kTiles / 2];
 #pragma unroll
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(kWaves * 64)
         if (!whole) {
 #pragma unroll
           for (int x = 0; x < kTiles; ++x) {
-            const bool here = lds.present[buf][x] != 0;
+            const bool here = !(flags >> 8 * x & kAbsent);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               st[y][x][r] =
@@ -171,10 +178,9 @@ __global__ void __launch_bounds__(kWaves * 64)
         for (int x = 0; x < kTiles; ++x)
 #pragma unroll
           for (int r = 0; r < 4; ++r) top = fmaxf(top, st[y][x][r]);
-        top = max_over_groups(top);
-        if (__any(top > m[y])) {
-          const float alpha =
-              __builtin_amdgcn_exp2f((m[y] - (top == kNegInf ? 0.0f : top)) * a.scale);
+        if (__any(outgrown(a, top, m[y]))) {
+          top = max_over_groups(top);
+          const float alpha = rescale(a, top, m[y]);
           m[y] = top;
           l[y] *= alpha;
 #pragma unroll
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(kWaves * 64)
           for (int y = 0; y < kRT; ++y)
             o[y][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[y][h], o[y][d], 0, 0, 0);
         }
-      if (nan) {
+      if (flags & kNan * kEveryTile) {
         for (int x = 0; x < kTiles; ++x)
 #pragma unroll
           for (int c = 0; c < Codes::kScales; ++c)
