@@ -220,6 +220,7 @@ int check_attention(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk
   a->q_head = q->stride1;
   a->group = (int)(q->dim1 / heads);
   a->window = (int)std::min<int64_t>(params->window, kKv4MaxLength);
+  a->span = a->window ? (uint32_t)a->window : 1u << 31;
   a->sinks = a->window ? (int)std::min<int64_t>(params->sinks, kKv4MaxLength) : 0;
   a->scale = (float)((double)params->scale * 1.4426950408889634);  // log2(e)
   *empty = batch->tokens == 0 || batch->sequences == 0;

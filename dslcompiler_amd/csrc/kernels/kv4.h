@@ -50,6 +50,7 @@ struct Kv4AttentionArgs {
   float* part;        // split partials: see kv4_attention.hip
   int group;          // query heads to a key head
   int window, sinks;  // window 0: none
+  uint32_t span;      // the window, or 2^31
   int tiles;          // row tiles (of all sequences)
   int splits, chunk;  // splits of a sequence's key steps, steps to a split
   float scale;        // of q.k, times log2(e)

@@ -166,17 +166,23 @@ struct TileCodes {
   }
 };
 
-// V of 32 keys in LDS, as bf16: [16-key tile][D / 16][half: 8 values][16 keys]
-// of 16 bytes, the keys of the second half swapped by 8 so that the 32 lanes
-// of a half wave, which read both halves of 8 keys, meet all 64 banks.
+// V of 16-key tiles in LDS, as bf16: [16-key tile][D / 16][half: 8 values][16
+// keys] of 16 bytes, the keys of the second half swapped by 8 and those of every
+// other 16 values by 4, so that the 32 lanes of a half wave, which read both
+// halves of 8 keys' 16 values or of 4 keys' 32, meet all 64 banks.
 template <int D>
 __device__ __forceinline__ int v_chunk(int x, int d16, int half, int key) {
-  return ((x * (D / 16) + d16) * 2 + half) * 256 + (key ^ (half * 8)) * 16;
+  return ((x * (D / 16) + d16) * 2 + half) * 256 + (key ^ (half * 8) ^ ((d16 & 1) * 4)) * 16;
 }
 
-// Whether the query at position pos sees key j (of a page that exists).
+// Whether the query at position pos sees key j (of a page that exists): among
+// the last a.span keys up to its own (all, without a window: pos - j, unsigned,
+// is at least 2^31 for a later key), or as one of the first.
+__device__ __forceinline__ bool in_window(const Kv4AttentionArgs& a, int pos, int j) {
+  return (uint32_t)(pos - j) < a.span;
+}
 __device__ __forceinline__ bool sees(const Kv4AttentionArgs& a, int pos, int j) {
-  return j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+  return in_window(a, pos, j) || (j <= pos && j < a.sinks);
 }
 
 // Values of NaN blocks go into the products as zeros (0 * NaN would reach the

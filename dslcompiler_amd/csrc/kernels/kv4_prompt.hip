@@ -1,37 +1,47 @@
 // kv4_prompt.hip -- attention over the 4-bit cache for many rows (prompts and
-// chunks of them): see kv4_attention.hip for the mathematics and the operands'
-// order.
+// chunks of them): the mathematics of kv4_attention.hip on 32 x 32 tiles
+// (v_mfma_f32_32x32x16_bf16).
 //
-// A workgroup's 4 waves share 128 rows, 32 each, and step through the same
-// keys, 64 at a time: every wave converts 16 keys and values from codes to bf16
-// into LDS, where all four read them as operands.  Two buffers, so one barrier
-// a step, and the codes of the step after next are on their way meanwhile.
+// Four waves share 128 rows, 32 each, and step through the same keys, 64 at a
+// time: every wave converts 16 keys and values from codes to bf16 into LDS,
+// where all four read them as operands, while the next step's codes are on their
+// way.
+#include <type_traits>
+
 #include "kv4_attention.h"
 
 namespace llk_gfx950 {
 namespace {
 
-constexpr int kWaves = 4, kRT = 2, kRows = kKv4PromptRows, kTiles = 4;
+constexpr int kRows = kKv4PromptRows, kTiles = 4;  // 16-key tiles of a step = waves of a group
 constexpr int kStep = 16 * kTiles;
-static_assert(kRows == kWaves * kRT * 16 && kStep == kv4_step(kRows), "row tile");
-
-constexpr uint8_t kAbsent = 1, kNan = 2;
-constexpr uint32_t kEveryTile = 0x01010101u;  // times a flag: that flag of every tile
+static_assert(kRows == kTiles * 32 && kStep == kv4_step(kRows), "row tile");
 
 template <int D>
 struct PromptLds {
-  uint8_t k[2][kStep * D * 2];  // [16-key tile][D / 32][64 lanes] of 16 bytes: A operands
-  uint8_t v[2][kStep * D * 2];  // v_chunk
-  // of each 16-key tile: lanes that hold part of a NaN block, and what a step
-  // looks at first, kAbsent (its page does not exist) and kNan
-  uint64_t nan[2][kTiles][TileCodes<D>::kScales];
-  uint8_t flags[2][kTiles];
+  uint8_t k[kStep * D * 2];  // [32 keys][D / 16][64 lanes] of 16 bytes: A operands
+  uint8_t v[kStep * D * 2];  // v_chunk
+  // of each 16-key tile: lanes that hold part of a NaN block of V; bit 0 of
+  // the flags: its page does not exist, bit 1: there is such a lane
+  uint64_t nan[kTiles][TileCodes<D>::kScales];
+  uint32_t flags[kTiles];
 };
 
+__device__ __forceinline__ float swap_max(float x) {  // over lane and lane ^ 32
+  const auto r =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap_sum(float x) {
+  const auto r =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 template <int D>
-__global__ void __launch_bounds__(kWaves * 64)
+__global__ void __launch_bounds__(kTiles * 64)
     __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) kv4_prompt_kernel(Kv4AttentionArgs a) {
-  constexpr int kD16 = D / 16, kJ = D / 32;
+  constexpr int kU = D / 16, kD32 = D / 32, kJ = D / 32;
   __shared__ __attribute__((aligned(16))) PromptLds<D> lds;
   using Codes = TileCodes<D>;
   const int lane = threadIdx.x & 63;
@@ -48,56 +58,59 @@ __global__ void __launch_bounds__(kWaves * 64)
   if (split >= used) return;
   const int begin = split * a.chunk;
   const int end = split == used - 1 ? rt.steps : begin + a.chunk;
-  const int col = lane & 15, grp = lane >> 4;
+  // a lane's row of S^T and O^T, and which 4 of every 8 keys (values) it holds;
+  // its token and group of the codes
+  const int lrow = lane & 31, half = lane >> 5, col = lane & 15;
 
-  // Q: the lane's row of each of the wave's 16-row tiles
-  const int wrow = wave * kRT * 16;
-  bf16x8 q[kRT][kJ];
-  int pos[kRT];
+  bf16x8 q[kU];
+  int pos;
+  {
+    const int r = wave * 32 + lrow, row = rt.row0 + (r < rt.rows ? r : 0);
+    const int token = row / a.group, qhead = head * a.group + row % a.group;
+    pos = min(rt.first + token, rt.p_hi);
+    const uint16_t* src =
+        a.q + (int64_t)(rt.token0 + token) * a.q_token + (int64_t)qhead * a.q_head + half * 8;
 #pragma unroll
-  for (int y = 0; y < kRT; ++y) {
-    const int r = wrow + y * 16 + col;
-    const int row = rt.row0 + (r < rt.rows ? r : 0);
-    const int i = row / a.group, h = head * a.group + row % a.group;
-    pos[y] = min(rt.first + i, rt.p_hi);
-    const uint16_t* src = a.q + (int64_t)(rt.token0 + i) * a.q_token + (int64_t)h * a.q_head;
-#pragma unroll
-    for (int j = 0; j < kJ; ++j)
-      q[y][j] = __builtin_bit_cast(bf16x8, load16_any(src + Codes::element(j, lane)));
+    for (int u = 0; u < kU; ++u) q[u] = __builtin_bit_cast(bf16x8, load16_any(src + u * 16));
   }
   // positions of the wave's first and last row
-  const int last = min(wrow + kRT * 16, rt.rows) - 1;
-  const int w_lo = rt.first + (rt.row0 + wrow) / a.group;
-  const int w_hi = last < wrow ? -1 : min(rt.first + (rt.row0 + last) / a.group, rt.p_hi);
+  const int last = max(min(wave * 32 + 32, rt.rows) - 1, 0);
+  const int w_lo = rt.first + (rt.row0 + min(wave * 32, last)) / a.group;
+  const int w_hi = min(rt.first + (rt.row0 + last) / a.group, rt.p_hi);
 
-  f32x4 o[kRT][kD16];
-  float m[kRT], l[kRT];
+  f32x16 o[kD32];
+  float m = kNegInf, l = 0.0f;
 #pragma unroll
-  for (int y = 0; y < kRT; ++y) {
-    m[y] = kNegInf, l[y] = 0.0f;
+  for (int d = 0; d < kD32; ++d)
 #pragma unroll
-    for (int d = 0; d < kD16; ++d) o[y][d] = f32x4{0, 0, 0, 0};
-  }
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
   const int page_mask = (1 << a.cache.page_shift) - 1;
   const uint8_t* const base = a.cache.data + head * a.cache.head_bytes;
   const int32_t* const table = a.batch.table + rt.s * a.batch.table_stride;
+  // first key of the group's step after that at k0 (number `step`)
   auto key0 = [&](int step) { return (step < rt.sink ? step : step - rt.sink + rt.low) * kStep; };
-  // the wave's 16 keys of a step
-  auto fetch = [&](int step, Codes& c) {
-    const int key = key0(step) + 16 * wave;
-    int id = -1;
-    if (key <= rt.p_hi) id = table[key >> a.cache.page_shift];
-    c.present = id >= 0 && id < a.cache.pages;
-    if (c.present)
-      c.load(base + id * a.cache.page_stride + (int64_t)((key & page_mask) >> 4) * (17 * D), lane);
-    else
-      c.clear();
+  // The wave converts 16 keys of a step, from the tile at k0 + 16 wave.  Its page
+  // is asked for a step before its codes, by a vector load: a scalar one would
+  // have every LDS wait of the step wait for it.  Where there is no page, the
+  // codes are those of page 0, and no row sees them.
+  auto page_of = [&](int k0) {
+    const int key = k0 + 16 * wave;
+    return key <= rt.p_hi ? __builtin_nontemporal_load(table + (key >> a.cache.page_shift)) : -1;
   };
-  auto place = [&](int step, int buf, const Codes& c) {
-    const bool past = key0(step) + 16 * wave + col > rt.p_hi;
+  auto fetch = [&](int k0, int page, Codes& c) {
+    const int id = __builtin_amdgcn_readfirstlane(page);
+    c.present = id >= 0 && id < a.cache.pages;
+    c.load(base + (c.present ? id : 0) * a.cache.page_stride +
+               (((k0 + 16 * wave) & page_mask) >> 4) * (17 * D), lane);
+  };
+  // where the lane's first 8 values go
+  const int kto = (((wave >> 1) * kU + (Codes::element(0, lane) >> 4)) * 64 +
+                   (Codes::element(0, lane) >> 3 & 1) * 32 + (wave & 1) * 16 + col) * 16;
+  uint64_t nan[Codes::kScales];
+  auto place = [&](int k0, const Codes& c) {
+    const bool past = !c.present || k0 + 16 * wave + col > rt.p_hi;
     float ks[Codes::kScales], vs[Codes::kScales];
-    uint64_t nan[Codes::kScales];
 #pragma unroll
     for (int i = 0; i < Codes::kScales; ++i) {
       const uint32_t e = past ? 0u : c.vs[i];
@@ -107,149 +120,172 @@ __global__ void __launch_bounds__(kWaves * 64)
     }
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      *reinterpret_cast<bf16x8*>(lds.k[buf] + ((wave * kJ + j) * 64 + lane) * 16) =
-          decode8(c.k[j], ks[Codes::scale_of(j)]);
       const int d = Codes::element(j, lane);
-      *reinterpret_cast<bf16x8*>(lds.v[buf] + v_chunk<D>(wave, d >> 4, (d >> 3) & 1, col)) =
+      *reinterpret_cast<bf16x8*>(lds.k + kto + (Codes::element(j, 0) >> 4) * 1024 + (j & 1) * 512) =
+          decode8(c.k[j], ks[Codes::scale_of(j)]);
+      *reinterpret_cast<bf16x8*>(lds.v + v_chunk<D>(wave, d >> 4, j & 1, col)) =
           decode8(c.v[j], vs[Codes::scale_of(j)]);
     }
-    if (lane == 0) {
-      uint64_t any = 0;
+  };
+  // what the waves have to know of the tile placed last
+  auto note = [&](bool present) {
+    uint64_t any = 0;
 #pragma unroll
-      for (int i = 0; i < Codes::kScales; ++i) any |= lds.nan[buf][wave][i] = nan[i];
-      lds.flags[buf][wave] = (c.present ? 0 : kAbsent) | (any ? kNan : 0);
+    for (int i = 0; i < Codes::kScales; ++i) any |= nan[i];
+    if (lane == 0) {
+      lds.flags[wave] = (present ? 0 : 1) | (any ? 2 : 0);
+#pragma unroll
+      for (int i = 0; i < Codes::kScales; ++i) lds.nan[wave][i] = nan[i];
     }
   };
 
+  // First keys of this step and the next two: the codes of the one and the page
+  // of the other are on their way.
   Codes codes;
-  if (begin < end) {
-    fetch(begin, codes);
-    place(begin, 0, codes);
-    if (begin + 1 < end) fetch(begin + 1, codes);
-  }
-  __syncthreads();
-  for (int step = begin; step < end; ++step) {
-    const int buf = (step - begin) & 1;
-    const int k0 = key0(step);
-    // some row of the wave sees some key of the step
-    const bool any = k0 <= w_hi &&
-                     (!a.window || k0 + kStep - 1 > w_lo - a.window || k0 < a.sinks);
-    if (any) {
-      const uint32_t flags = __builtin_amdgcn_readfirstlane(
-          *reinterpret_cast<const uint32_t*>(lds.flags[buf]));
+  int k0 = key0(begin), k1 = key0(begin + 1);
+  fetch(k0, page_of(k0), codes);
+  int page = page_of(k1);
+  // Where the lane's operands lie in a buffer: K, and V's two halves (v_chunk's
+  // swap apart, a constant step from one 32 values to the next).
+  const int vkey = 4 * half + (col >> 2), vhalf = (col >> 1) & 1, vsub = (lane >> 4) & 1;
+  const int kat = lane * 16;
+  const int vat[2] = {v_chunk<D>(0, vsub, vhalf, vkey) + (col & 1) * 8,
+                      v_chunk<D>(0, vsub, vhalf, vkey + 8) + (col & 1) * 8};
+  // One step.
+  auto work = [&] {
+    const u32x4 tile_flags = *reinterpret_cast<const u32x4*>(lds.flags);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {  // 32 keys each
+      f32x16 st;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st[e] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        st = mfma32(*reinterpret_cast<const bf16x8*>(lds.k + kat + (x * kU + u) * 1024), q[u], st);
+      const int j0 = k0 + 32 * x;
+      const uint32_t flags =
+          __builtin_amdgcn_readfirstlane(tile_flags[2 * x] | tile_flags[2 * x + 1]);
       // every row sees every key
-      const bool whole = k0 + kStep - 1 <= w_lo && !(flags & kAbsent * kEveryTile) &&
-                         (!a.window || k0 > w_hi - a.window || k0 + kStep <= a.sinks);
-      f32x4 st[kRT][kTiles];
-      bf16x8 k[2][kJ];  // of this tile, and of the next, on its way
-      auto read_k = [&](int x) {
+      const bool whole = j0 + 31 <= w_lo && !(flags & 1) &&
+                         (!a.window || j0 > w_hi - a.window || j0 + 32 <= a.sinks);
+      if (!whole) {
+        auto mask = [&](auto first) {
 #pragma unroll
-        for (int j = 0; j < kJ; ++j)
-          k[x & 1][j] =
-              *reinterpret_cast<const bf16x8*>(lds.k[buf] + ((x * kJ + j) * 64 + lane) * 16);
-      };
-      read_k(0);
-#pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        if (x + 1 < kTiles) read_k(x + 1);
-#pragma unroll
-        for (int y = 0; y < kRT; ++y) st[y][x] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < kJ; ++j)
-#pragma unroll
-          for (int y = 0; y < kRT; ++y)
-            st[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[x & 1][j], q[y][j], st[y][x], 0, 0, 0);
-      }
-      bf16x8 p[kRT][kTiles / 2];
-#pragma unroll
-      for (int y = 0; y < kRT; ++y) {
-        if (!whole) {
-#pragma unroll
-          for (int x = 0; x < kTiles; ++x) {
-            const bool here = !(flags >> 8 * x & kAbsent);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              st[y][x][r] =
-                  here && sees(a, pos[y], k0 + 16 * x + 4 * grp + r) ? st[y][x][r] : kNegInf;
+          for (int e = 0; e < 16; ++e) {
+            const int j = j0 + 8 * (e >> 2) + 4 * half + (e & 3);
+            st[e] = in_window(a, pos, j) || (first && j <= pos && j < a.sinks) ? st[e] : kNegInf;
           }
-        }
-        float top = m[y];
+        };
+        if (j0 < a.sinks) mask(std::true_type{});
+        else mask(std::false_type{});
+        if (flags & 1) {
 #pragma unroll
-        for (int x = 0; x < kTiles; ++x)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, st[y][x][r]);
-        if (__any(outgrown(a, top, m[y]))) {
-          top = max_over_groups(top);
-          const float alpha = rescale(a, top, m[y]);
-          m[y] = top;
-          l[y] *= alpha;
-#pragma unroll
-          for (int d = 0; d < kD16; ++d) o[y][d] *= alpha;
-        }
-        const float shift = m[y] == kNegInf ? 0.0f : m[y] * a.scale;
-#pragma unroll
-        for (int h = 0; h < kTiles / 2; ++h) {
-          float e[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(
-                __builtin_fmaf(st[y][2 * h + (i >> 2)][i & 3], a.scale, -shift));
-            l[y] += e[i];
-          }
-          p[y][h] = __builtin_bit_cast(
-              bf16x8, u32x4{f32x2_to_bf16x2_rne(e[0], e[1]), f32x2_to_bf16x2_rne(e[2], e[3]),
-                            f32x2_to_bf16x2_rne(e[4], e[5]), f32x2_to_bf16x2_rne(e[6], e[7])});
+          for (int e = 0; e < 16; ++e)
+            st[e] = tile_flags[2 * x + (e >> 3)] & 1 ? kNegInf : st[e];
         }
       }
-      const int vkey = 4 * grp + (col >> 2), vhalf = (col >> 1) & 1;
+      // Keeps the scores in their registers: the compiler would take the tuple
+      // apart here and copy its values on the way without a mask.
+      asm("" : "+v"(st));
+      float top = m;
 #pragma unroll
-      for (int h = 0; h < kTiles / 2; ++h)
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, st[e]);
+      if (__any(outgrown(a, top, m))) {
+        top = swap_max(top);
+        const float alpha = rescale(a, top, m);
+        m = top;
+        l *= alpha;
 #pragma unroll
-        for (int d = 0; d < kD16; ++d) {
+        for (int d = 0; d < kD32; ++d) o[d] *= alpha;
+      }
+      const float shift = m == kNegInf ? 0.0f : m * a.scale;
+      bf16x8 p[2];  // of 16 keys each
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t two[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float e[2];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            e[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[g * 8 + 2 * i + n], a.scale, -shift));
+          l += e[0];
+          l += e[1];
+          two[i] = f32x2_to_bf16x2_rne(e[0], e[1]);
+        }
+        p[g] = __builtin_bit_cast(bf16x8, u32x4{two[0], two[1], two[2], two[3]});
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int d = 0; d < kD32; ++d) {
           v4i16 part[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            part[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_v4i16)(lds.v[buf] + v_chunk<D>(2 * h + x, d, vhalf, vkey) + (col & 1) * 8));
+          for (int y = 0; y < 2; ++y)
+            part[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_v4i16)(lds.v + vat[y] + ((2 * x + g) * kU + 2 * d) * 512));
           const bf16x8 v = __builtin_bit_cast(
               bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int y = 0; y < kRT; ++y)
-            o[y][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[y][h], o[y][d], 0, 0, 0);
+          o[d] = mfma32(v, p[g], o[d]);
         }
-      if (flags & kNan * kEveryTile) {
-        for (int x = 0; x < kTiles; ++x)
+    }
+    if (__builtin_amdgcn_readfirstlane(tile_flags[0] | tile_flags[1] | tile_flags[2] |
+                                       tile_flags[3]) & 2) {  // rare: see add_nan
+      for (int g = 0; g < kTiles; ++g) {
+        uint32_t seen = 0;
+#pragma unroll 1
+        for (int j = 0; j < 16; ++j) seen |= (uint32_t)sees(a, pos, k0 + 16 * g + j) << j;
 #pragma unroll
-          for (int c = 0; c < Codes::kScales; ++c)
-#pragma unroll
-            for (int y = 0; y < kRT; ++y)
-              add_nan<D>(a, lds.nan[buf][x][c], c, k0 + 16 * x, pos[y], o[y]);
+        for (int d = 0; d < kD32; ++d) {
+          // a lane holds values of one block (32 d on) in every register of o[d]
+          const int c = D == 256 ? d >> 2 : 0;
+          const uint64_t f = lds.nan[g][c];
+          const uint32_t part = D == 64 ? (uint32_t)(f >> (32 * d)) | (uint32_t)(f >> (32 * d + 16))
+                                        : (uint32_t)(f >> (16 * (d & 3)));
+          if (part & seen & 0xffffu) o[d] += __builtin_nanf("");
+        }
       }
     }
-    if (step + 1 < end) {
-      place(step + 1, buf ^ 1, codes);
-      if (step + 2 < end) fetch(step + 2, codes);
-    }
+  };
+  for (int step = begin; step < end; ++step) {
+    __syncthreads();  // every wave is done with the step before
+    place(k0, codes);
+    note(codes.present);
+    fetch(k1, page, codes);
+    const int k2 = key0(step + 2);
+    page = page_of(k2);
     __syncthreads();
+    // some row of the wave sees some key of the step
+    if (k0 <= w_hi && (!a.window || k0 + kStep - 1 > w_lo - a.window || k0 < a.sinks)) work();
+    k0 = k1, k1 = k2;
   }
 
-  float* const part = used > 1 ? part_of<D, kRows>(a, tile, head, split) : nullptr;
+  l = swap_sum(l);
+  const int r = wave * 32 + lrow;
+  if (r >= rt.rows) return;
+  const int token = (rt.row0 + r) / a.group;
+  const int qhead = head * a.group + (rt.row0 + r) % a.group;
+  // the lane's values: 32 d + 8 e + 4 half on
+  if (used > 1) {
+    float* const part = part_of<D, kRows>(a, tile, head, split);
+    if (half == 0) part[kRows * D + r] = m, part[kRows * (D + 1) + r] = l;
 #pragma unroll
-  for (int y = 0; y < kRT; ++y) {
-    const int r = wrow + y * 16 + col;
-    Joined sum(m[y]);
-    sum.l = sum_over_groups(l[y]);
-    if (r >= rt.rows) continue;
-    if (part && grp == 0) part[kRows * D + r] = sum.m, part[kRows * (D + 1) + r] = sum.l;
+    for (int d = 0; d < kD32; ++d)
 #pragma unroll
-    for (int d = 0; d < kD16; ++d) {
-      if (part) {
-        *reinterpret_cast<f32x4*>(part + r * D + d * 16 + 4 * grp) = o[y][d];
-      } else {
-        sum.o = o[y][d];
-        sum.store(a, rt, head, r, d * 16 + 4 * grp);
-      }
-    }
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(part + r * D + d * 32 + e * 8 + 4 * half) =
+            f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+  } else {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* const dst = a.out + (int64_t)(rt.token0 + token) * a.out_token +
+                          (int64_t)qhead * a.out_head + 4 * half;
+#pragma unroll
+    for (int d = 0; d < kD32; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        store8_any(dst + d * 32 + e * 8,
+                   make_uint2(f32x2_to_bf16x2_rne(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
+                              f32x2_to_bf16x2_rne(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)));
   }
 }
 
@@ -259,7 +295,7 @@ hipError_t prompt(const Kv4AttentionArgs& args, hipStream_t s) {
   void* params[] = {&a};
   return hipLaunchKernel(reinterpret_cast<const void*>(&kv4_prompt_kernel<D>),
                          dim3((unsigned)(a.tiles * a.cache.heads), (unsigned)a.splits),
-                         dim3(kWaves * 64), params, 0, s);
+                         dim3(kTiles * 64), params, 0, s);
 }
 
 }  // namespace
