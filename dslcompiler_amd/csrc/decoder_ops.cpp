@@ -190,7 +190,7 @@ AttentionPlan plan_attention(const Kv4Batch& b, int page_shift, int heads, int g
                                          (window + p.rows / group + step - 1) / step + 2);
   const int64_t groups = p.tiles * heads;
   int64_t s = p.rows == kKv4PromptRows ? std::max<int64_t>(1, 512 / groups)
-                                      : (1024 + groups - 1) / groups;
+                                      : std::min<int64_t>(128, (2048 + groups - 1) / groups);
   s = std::min<int64_t>(s, std::max<int64_t>(1, steps / 8));
   p.chunk = (int)std::max<int64_t>(1, (steps + s - 1) / s);
   p.splits = (int)std::max<int64_t>(1, (steps + p.chunk - 1) / p.chunk);

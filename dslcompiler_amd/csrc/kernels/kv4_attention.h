@@ -120,6 +120,14 @@ __device__ __forceinline__ bf16x8 decode8(uint32_t codes, float scale) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <bool ONCE, class T>
+__device__ __forceinline__ T read(const uint8_t* p) {
+  const T* q = reinterpret_cast<const T*>(p);
+  if constexpr (ONCE) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+
 // One lane's share of a 16-token tile: D / 4 keys' codes and values' codes of
 // token lane % 16 -- the contiguous D / 4 values from lane / 16 * D / 4 (D =
 // 256: from 32 (lane / 16) and 128 + 32 (lane / 16)) -- and their scales.
@@ -131,32 +139,28 @@ struct TileCodes {
   uint32_t ks[kScales], vs[kScales];  // scale bytes
   int present;                        // the tile's page exists
 
+  // ONCE: no other workgroup reads the tile, so it need not stay in L2.
+  template <bool ONCE>
   __device__ __forceinline__ void load(const uint8_t* tile, int lane) {
     if constexpr (D == 64) {
       const int block = lane >> 5, half = (lane >> 4) & 1, tok = lane & 15;
       const int at = (block * 16 + tok) * 16 + half * 8;
-      const uint2 a = *reinterpret_cast<const uint2*>(tile + at);
-      const uint2 b = *reinterpret_cast<const uint2*>(tile + 8 * D + at);
-      k[0] = a.x, k[1] = a.y, v[0] = b.x, v[1] = b.y;
+      const u32x2 a = read<ONCE, u32x2>(tile + at), b = read<ONCE, u32x2>(tile + 8 * D + at);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) k[i] = a[i], v[i] = b[i];
       ks[0] = tile[16 * D + block * 16 + tok];
       vs[0] = tile[16 * D + D / 2 + block * 16 + tok];
     } else {
 #pragma unroll
       for (int c = 0; c < kScales; ++c) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(tile + c * 1024 + lane * 16);
-        const u32x4 b = *reinterpret_cast<const u32x4*>(tile + 8 * D + c * 1024 + lane * 16);
+        const u32x4 a = read<ONCE, u32x4>(tile + c * 1024 + lane * 16);
+        const u32x4 b = read<ONCE, u32x4>(tile + 8 * D + c * 1024 + lane * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) k[4 * c + i] = a[i], v[4 * c + i] = b[i];
         ks[c] = tile[16 * D + c * 64 + lane];
         vs[c] = tile[16 * D + D / 2 + c * 64 + lane];
       }
     }
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < kDwords; ++i) k[i] = v[i] = 0;
-#pragma unroll
-    for (int i = 0; i < kScales; ++i) ks[i] = vs[i] = 0;
   }
   static __device__ __forceinline__ int scale_of(int dword) { return D == 256 ? dword / 4 : 0; }
   // First of the 8 values of dword j.

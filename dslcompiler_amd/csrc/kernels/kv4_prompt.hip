@@ -101,8 +101,9 @@ __global__ void __launch_bounds__(kTiles * 64)
   auto fetch = [&](int k0, int page, Codes& c) {
     const int id = __builtin_amdgcn_readfirstlane(page);
     c.present = id >= 0 && id < a.cache.pages;
-    c.load(base + (c.present ? id : 0) * a.cache.page_stride +
-               (((k0 + 16 * wave) & page_mask) >> 4) * (17 * D), lane);
+    c.template load<false>(base + (c.present ? id : 0) * a.cache.page_stride +
+                               (((k0 + 16 * wave) & page_mask) >> 4) * (17 * D),
+                           lane);
   };
   // where the lane's first 8 values go
   const int kto = (((wave >> 1) * kU + (Codes::element(0, lane) >> 4)) * 64 +
