@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(BlockNormArgs a) {
   const int64_t yo = m * a.ldy, ho = m * a.ldh, go = m * a.ldg;
   Chunk<YF> y[CH], g[CH];
   Chunk<RF> h[CH];
+  Chunk<WF> wpost[CH], wpre[CH];
   int c[CH], n[CH];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
@@ -109,6 +110,13 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(BlockNormArgs a) {
     h[k].load(a.h, ho + 8 * c[k], n[k]);
     if (a.y) y[k].load(a.y, yo + 8 * c[k], n[k]);
     if (a.g) g[k].load(a.g, go + 8 * c[k], n[k]);
+  }
+  // the weights too before the first sum, not each after its own
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    if (n[k] == 0) continue;
+    if (a.wpost) wpost[k].load(a.wpost, 8 * c[k], n[k]);
+    wpre[k].load(a.wpre, 8 * c[k], n[k]);
   }
   float r = 1.0f;
   if (a.wpost) {
@@ -125,14 +133,12 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(BlockNormArgs a) {
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     if (n[k] == 0) continue;
-    Chunk<WF> w;
-    if (a.wpost) w.load(a.wpost, 8 * c[k], n[k]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float x = h[k].get(i);
       if (a.y) {
         float u = y[k].get(i);
-        if (a.wpost) u = u * r * (w.get(i) + a.offset);
+        if (a.wpost) u = u * r * (wpost[k].get(i) + a.offset);
         if (a.g) u *= g[k].get(i);
         x = __builtin_fmaf(a.scale, u, x);
       }
@@ -146,10 +152,8 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(BlockNormArgs a) {
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     if (n[k] == 0) continue;
-    Chunk<WF> w;
-    w.load(a.wpre, 8 * c[k], n[k]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * r * (w.get(i) + a.offset);
+    for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * r * (wpre[k].get(i) + a.offset);
     Chunk<OF>::store(a.out, m * a.ldo + 8 * c[k], n[k], v[k]);
   }
 }
@@ -176,9 +180,11 @@ hipError_t llk_launch_block_norm(const BlockNormArgs& a, int64_t M, bool y_f32, 
                                  bool o_f32, bool w_f32, hipStream_t s) {
   using namespace llk_gfx950;
   const int chunks = (a.N + 7) / 8;
-  // The fewest chunks per thread that 1024 threads hold.
-  int ch = 1;
-  while (ch < 4 && chunks > ch * 256) ch *= 2;
+  // Chunks to a thread: one where few rows leave CUs idle (17 x 5120: 6.3 us,
+  // with two 6.9), two where there are enough (4097 x 5120 with a gate, bf16: 47
+  // us, with one 54); more only where 1024 threads are too few.
+  int ch = M <= 512 ? 1 : 2;
+  while (chunks > ch * 1024) ch *= 2;
   const int threads = ((chunks + ch - 1) / ch + 63) / 64 * 64;
   const void* fn = ch == 1   ? pick<1>(y_f32, h_f32, o_f32, w_f32)
                    : ch == 2 ? pick<2>(y_f32, h_f32, o_f32, w_f32)

@@ -128,10 +128,13 @@ def block_norm(y, residual, pre_weight, *, post_weight=None, gate=None, scale: f
         od = _lib.Tensor2D(residual_out.data_ptr(), rd.dim0, n, n, 1)
     if out is None:
         out = _result(residual, out_dtype or _torch().bfloat16)
+        nd = _lib.Tensor2D(out.data_ptr(), rd.dim0, n, n, 1)
+    else:
+        nd = _rows(out, "out")
     params = _lib.BlockNormParams(ytype, rtype, _kind(out, "out", dev, _FLOATS), wtype, post,
                                   _weight(pre_weight, "pre_weight", n), gd, scale, eps,
                                   weight_offset)
-    check(lib().llk_block_norm(yd, rd, od, _rows(out, "out"), params, _context(dev, stream)))
+    check(lib().llk_block_norm(yd, rd, od, nd, params, _context(dev, stream)))
     return residual_out, out
 
 
@@ -215,7 +218,7 @@ def kv4_read(cache, table, lens, *, head_dim: int, starts=None, tokens: int | No
     batch = _batch(table, lens, starts, tokens, None, dev)
     if k is None:
         torch = _torch()
-        k = torch.empty((tokens, cd.heads, head_dim), dtype=torch.bfloat16, device=cache.device)
+        k = cache.new_empty((tokens, cd.heads, head_dim), dtype=torch.bfloat16)
         if v is None:
             v = torch.empty_like(k)
     elif v is None:
@@ -248,7 +251,11 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
     args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev)
     if out is None:
         out = _result(q, q.dtype)
-    check(lib().llk_kv4_attention(*args, _rows3(out, "out", dev), _context(dev, stream, scratch)))
+        qd = args[0]
+        od = _lib.Tensor3D(out.data_ptr(), qd.dim0, qd.dim1, qd.dim2, qd.dim1 * qd.dim2, qd.dim2, 1)
+    else:
+        od = _rows3(out, "out", dev)
+    check(lib().llk_kv4_attention(*args, od, _context(dev, stream, scratch)))
     return out
 
 
