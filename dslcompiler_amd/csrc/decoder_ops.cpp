@@ -158,7 +158,8 @@ int check_move(const llk_tensor3d* k, const llk_tensor3d* v, const llk_kv4_cache
       (rc = check_rows3(v, "v", b->tokens, c->heads, cache->head_dim, result)))
     return rc;
   *r = Kv4Rows{bf16_of(k), bf16_of(v), k->stride0, k->stride1, v->stride0, v->stride1};
-  *empty = b->tokens == 0 || b->sequences == 0;
+  // (a read without sequences gives zeros)
+  *empty = b->tokens == 0 || (b->sequences == 0 && !result);
   int dev;
   return *empty ? LLK_OK : llk::current_gfx950(&dev);
 }

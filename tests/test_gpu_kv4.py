@@ -188,6 +188,23 @@ def test_tokens_without_a_place(llk, gpu):
         assert (got[held] == 1).all() and (got[~held] == 0).all()
 
 
+def test_no_sequences(llk, gpu):
+    """Rows that belong to no sequence at all: nothing written, zeros read."""
+    pool = llk.kv4_cache(2, 2, 16, 64)
+    pool.fill_(7)
+    table = gpu.zeros((0, 3), dtype=gpu.int32, device="cuda")
+    lens = gpu.zeros(0, dtype=gpu.int32, device="cuda")
+    starts = gpu.zeros(1, dtype=gpu.int32, device="cuda")
+    x = gpu.ones((5, 2, 64), dtype=gpu.bfloat16, device="cuda")
+    llk.kv4_write(x, x, pool, table, lens, starts=starts)
+    assert bool((pool == 7).all())
+    k, v = x.clone(), x.clone()
+    llk.kv4_read(pool, table, lens, head_dim=64, starts=starts, k=k, v=v)
+    assert bool((k == 0).all()) and bool((v == 0).all())
+    out = llk.kv4_attention(x, pool, table, lens, starts=starts)
+    assert out.shape == x.shape
+
+
 def test_write_read_strides(llk, gpu):
     """Keys and values as slices at odd elements and with heads outermost; a
     cache that is one layer of a larger pool; results into a wider buffer."""
