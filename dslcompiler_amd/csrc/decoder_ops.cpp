@@ -179,7 +179,13 @@ AttentionPlan plan_attention(const Kv4Batch& b, int page_shift, int heads, int g
   AttentionPlan p{};
   const int64_t rows_each = b.starts ? ((int64_t)b.tokens * group + b.sequences - 1) / b.sequences
                                      : group;
-  p.rows = rows_each <= 16 ? 16 : rows_each <= 32 ? 32 : kKv4PromptRows;
+  // Tiles of 16 and 32 rows read the keys once more per tile and split them over
+  // the chip; one of 128 rows converts each key once for 4 waves, and pays when
+  // it is full.  Measured, D = 128, context 8000, us: 16 rows a sequence, 16
+  // sequences: 37 by 16 rows, 48 by 32; 24 on average: 52 by 32, 121 by 128; 96:
+  // 117 and 166; 128, one sequence: 28.6 and 26.6; 256, 16 sequences: 187 both
+  // (context 1000: 93 and 33).
+  p.rows = rows_each <= 16 ? 16 : rows_each <= 96 ? 32 : kKv4PromptRows;
   p.tiles = b.starts ? (int64_t)b.tokens * group / p.rows + b.sequences
                      : (int64_t)b.sequences * ((group + p.rows - 1) / p.rows);
   int64_t len = std::min<int64_t>((int64_t)b.table_pages << page_shift, kKv4MaxLength);
@@ -190,9 +196,19 @@ AttentionPlan plan_attention(const Kv4Batch& b, int page_shift, int heads, int g
     steps = std::min<int64_t>(steps, (sinks + step - 1) / step +
                                          (window + p.rows / group + step - 1) / step + 2);
   const int64_t groups = p.tiles * heads;
-  int64_t s = p.rows == kKv4PromptRows ? std::max<int64_t>(1, 512 / groups)
-                                      : std::min<int64_t>(128, (2048 + groups - 1) / groups);
-  s = std::min<int64_t>(s, std::max<int64_t>(1, steps / 8));
+  // Splits of the keys: enough workgroups for the chip, none of a few steps only,
+  // since a second kernel joins them.  Measured, us: tiles of 128 rows, 64 groups
+  // at 8000 keys, about 512 workgroups 67, 256 85, 1024 75.  Smaller tiles, 512
+  // groups at 8000 keys, 4 splits 78, 8 79, 15 86; 64 groups at 2000, 7 splits 13.2,
+  // 3 14.2; 512 groups at 500, one 12.2, two 17.1; 8 groups at 30000 (16 rows),
+  // 63 splits 20.8, 105 24.9.
+  int64_t s;
+  if (p.rows == kKv4PromptRows)
+    s = std::min<int64_t>(std::max<int64_t>(1, 512 / groups), steps / 8);
+  else
+    s = std::min<int64_t>(std::min<int64_t>(64, (2048 + groups - 1) / groups),
+                          steps / (groups >= 256 ? 16 : 8));
+  s = std::max<int64_t>(s, 1);
   p.chunk = (int)std::max<int64_t>(1, (steps + s - 1) / s);
   p.splits = (int)std::max<int64_t>(1, (steps + p.chunk - 1) / p.chunk);
   p.bytes = llk_kv4_attention_part_bytes(p.tiles, heads, p.splits, p.rows, D);
