@@ -279,6 +279,43 @@ def test_long_sequences_are_split(llk, gpu):
     check(*attend(llk, c, c.queries(4)))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64, 512])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 1), (33, 0), (64, 40), (200, 64), (16, 5000)])
+def test_full_row_tiles(llk, gpu, D, page, window, sinks):
+    """Rows enough for the tiles of 128, of which each sequence's last is part."""
+    c = Case(gpu, [300, 130, 511, 1], [130, 130, 1, 1], 1, D, page, seed=D + window)
+    q = c.queries(3)
+    pool, table, lens, starts = c.dev()
+    plan = llk.describe_kv4_attention(_dev(gpu, q, gpu.bfloat16), pool, table, lens, starts=starts)
+    assert plan["rows"] == 128
+    check(*attend(llk, c, q, window=window, sinks=sinks))
+    # tiles by the rows of a sequence on average, the same rows in both
+    for new, rows in ((96, 32), (97, 128)):
+        c = Case(gpu, [200, 100], [new, new], 1, D, page, seed=new)
+        q = c.queries(1)
+        pool, table, lens, starts = c.dev()
+        plan = llk.describe_kv4_attention(_dev(gpu, q, gpu.bfloat16), pool, table, lens,
+                                          starts=starts)
+        assert plan["rows"] == rows
+        check(*attend(llk, c, q, window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_over_a_long_context_is_split(llk, gpu, D):
+    c = Case(gpu, [3000, 1700, 140], [130, 100, 120], 1, D, 64, seed=D)
+    c.table[0, 20] = -1  # a page given back
+    q = c.queries(1)
+    pool, table, lens, starts = c.dev()
+    plan = llk.describe_kv4_attention(_dev(gpu, q, gpu.bfloat16), pool, table, lens, starts=starts)
+    assert plan["rows"] == 128 and plan["splits"] > 1 and plan["launches"] == 2
+    got, want, mag = attend(llk, c, q)
+    check(got, want, mag)
+    for max_len in (1, 300, 1500):
+        check(attend(llk, c, q, max_len=max_len)[0], want, mag, max_len)
+    check(*attend(llk, c, q, window=1100, sinks=70))
+
+
 def test_large_scores(llk, gpu):
     """Scores of hundreds, where the running maximum moves late and far."""
     c = Case(gpu, [700, 64], [1, 30], 2, 128, 16, seed=4, big=4.0)
