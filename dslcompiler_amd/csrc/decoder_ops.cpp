@@ -197,17 +197,23 @@ AttentionPlan plan_attention(const Kv4Batch& b, int page_shift, int heads, int g
                                          (window + p.rows / group + step - 1) / step + 2);
   const int64_t groups = p.tiles * heads;
   // Splits of the keys: enough workgroups for the chip, none of a few steps only,
-  // since a second kernel joins them.  Measured, us: tiles of 128 rows, 64 groups
-  // at 8000 keys, about 512 workgroups 67, 256 85, 1024 75.  Smaller tiles, 512
-  // groups at 8000 keys, 4 splits 78, 8 79, 15 86; 64 groups at 2000, 7 splits 13.2,
-  // 3 14.2; 512 groups at 500, one 12.2, two 17.1; 8 groups at 30000 (16 rows),
-  // 63 splits 20.8, 105 24.9.
+  // since a second kernel joins them.  Measured, D = 128, us.
   int64_t s;
-  if (p.rows == kKv4PromptRows)
-    s = std::min<int64_t>(std::max<int64_t>(1, 512 / groups), steps / 8);
-  else
+  if (p.rows == kKv4PromptRows) {
+    // About 512 workgroups, two to a CU: 64 groups at 8000 keys 60, by 256 85, by
+    // 1024 74; 256 groups of 4000 keys, 2 splits 91, 4 99.  Steps a split: 64
+    // groups at 1000 keys by 4 21, by 8 24, one split 30; 136 groups 31, 29 and
+    // 31; 256 groups, by 8 38, one split 32.
+    s = std::min<int64_t>(std::max<int64_t>(1, 512 / groups),
+                          steps / std::clamp<int64_t>(groups / 16, 4, 16));
+  } else {
+    // About 2048 workgroups: 512 groups at 8000 keys, 4 splits 78, 8 79, 15 86.
+    // At most 64: 8 groups at 30000 (16 rows) 20.8, 105 splits 24.9.  Steps a
+    // split: 64 groups at 2000, 7 splits 13.2, 3 14.2; 512 groups at 500, one
+    // split 12.2, two 17.1.
     s = std::min<int64_t>(std::min<int64_t>(64, (2048 + groups - 1) / groups),
                           steps / (groups >= 256 ? 16 : 8));
+  }
   s = std::max<int64_t>(s, 1);
   p.chunk = (int)std::max<int64_t>(1, (steps + s - 1) / s);
   p.splits = (int)std::max<int64_t>(1, (steps + p.chunk - 1) / p.chunk);

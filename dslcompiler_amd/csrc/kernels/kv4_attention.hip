@@ -277,40 +277,54 @@ __global__ void __launch_bounds__(kWaves * 64)
   }
 }
 
-// Joins the splits of one row: a workgroup per (tile, key head; row), its
-// threads over 4 of the D elements and every kGroups-th split.
-template <int D, int R>
+// Up to so many splits a row is joined by one group of threads (4 splits of 64
+// sequences, 4 rows each: 4.6 us, by a workgroup to a row 5.8; 2 of 1000 tokens of
+// 32 heads: the call 38 us, 72), more by a workgroup (64 splits: 22 us, 27).
+constexpr int kJoinAlone = 8;
+
+// Joins the splits of a row in their order.  A group of D / 4 threads takes 4 of
+// the D elements each; with ALONE a group has a row to itself, otherwise a
+// workgroup's groups share one row, each over every kGroups-th split.
+template <int D, int R, bool ALONE>
 __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4AttentionArgs a) {
   constexpr int kPlane = R * (D + 2), kChunks = D / 4, kGroups = 256 / kChunks;
-  __shared__ f32x4 other[kGroups][kChunks];
-  __shared__ float other_l[kGroups];
   const int head = blockIdx.x % a.cache.heads, tile = blockIdx.x / a.cache.heads;
-  const int r = blockIdx.y;
+  const int ch = threadIdx.x % kChunks, group = threadIdx.x / kChunks;
+  const int r = ALONE ? blockIdx.y * kGroups + group : blockIdx.y;
   RowTile rt;
   if (!row_tile<R>(a, tile, &rt) || r >= rt.rows) return;
   const int used = used_splits(a, rt.steps);
   if (used <= 1) return;
   const float* const part = part_of<D, R>(a, tile, head, 0);
-  const int ch = threadIdx.x % kChunks, group = threadIdx.x / kChunks;
   Joined sum(kNegInf);
-  for (int s = threadIdx.x & 63; s < used; s += 64)
-    sum.m = fmaxf(sum.m, part[s * kPlane + R * D + r]);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) sum.m = fmaxf(sum.m, __shfl_xor(sum.m, d));
-#pragma unroll 4
-  for (int s = group; s < used; s += kGroups) {
+  auto add = [&](int s) {
     const float* p = part + s * kPlane;
     sum.add(p[R * D + r], p[R * (D + 1) + r],
             reinterpret_cast<const f32x4*>(p)[r * kChunks + ch], a.scale);
-  }
-  other[group][ch] = sum.o;
-  if (ch == 0) other_l[group] = sum.l;
-  __syncthreads();
-  if (group) return;
+  };
+  if constexpr (ALONE) {
+#pragma unroll 4
+    for (int s = 0; s < used; ++s) sum.m = fmaxf(sum.m, part[s * kPlane + R * D + r]);
+#pragma unroll 4
+    for (int s = 0; s < used; ++s) add(s);
+  } else {
+    __shared__ f32x4 other[kGroups][kChunks];
+    __shared__ float other_l[kGroups];
+    for (int s = threadIdx.x & 63; s < used; s += 64)
+      sum.m = fmaxf(sum.m, part[s * kPlane + R * D + r]);
 #pragma unroll
-  for (int g = 1; g < kGroups; ++g) {
-    sum.l += other_l[g];
-    sum.o += other[g][ch];
+    for (int d = 32; d; d >>= 1) sum.m = fmaxf(sum.m, __shfl_xor(sum.m, d));
+#pragma unroll 4
+    for (int s = group; s < used; s += kGroups) add(s);
+    other[group][ch] = sum.o;
+    if (ch == 0) other_l[group] = sum.l;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) {
+      sum.l += other_l[g];
+      sum.o += other[g][ch];
+    }
   }
   sum.store(a, rt, head, r, ch * 4);
 }
@@ -319,9 +333,14 @@ template <int D, int R>
 hipError_t join(const Kv4AttentionArgs& args, hipStream_t s) {
   Kv4AttentionArgs a = args;
   void* params[] = {&a};
-  const unsigned rows = a.batch.starts ? R : std::min(R, a.group);
-  return hipLaunchKernel(reinterpret_cast<const void*>(&kv4_join_kernel<D, R>),
-                         dim3((unsigned)(a.tiles * a.cache.heads), rows), dim3(256), params, 0, s);
+  const int rows = a.batch.starts ? R : std::min(R, a.group);
+  constexpr int kGroups = 1024 / D;
+  const bool alone = a.splits <= kJoinAlone;
+  return hipLaunchKernel(alone ? reinterpret_cast<const void*>(&kv4_join_kernel<D, R, true>)
+                               : reinterpret_cast<const void*>(&kv4_join_kernel<D, R, false>),
+                         dim3((unsigned)(a.tiles * a.cache.heads),
+                              (unsigned)(alone ? (rows + kGroups - 1) / kGroups : rows)),
+                         dim3(256), params, 0, s);
 }
 
 template <int D, int RT>

@@ -7,12 +7,13 @@
 // where all four read them as operands, while the next step's codes are on their
 // way.
 //
-// Bound by the chain of one tile's steps, not by a unit: of ~3400 clocks a step
-// at D = 128 the matrix instructions take ~1000, converting and placing the codes
-// ~1000, softmax and barriers the rest.  One buffer of keys and values leaves
-// room for two workgroups to a CU, which fill each other's waits (2048 tokens of
-// 32 heads: 53 us, 650 TFLOP/s of what causality leaves; two buffers in turn, 8
-// waves, or 128 keys a step measured no less).
+// Bound by no one unit: at D = 128 a workgroup alone takes ~3500 clocks (1.7 us) a
+// step, of which its matrix instructions are 1024, and two on a CU, which is what
+// the registers leave room for, ~2100 each.  Matrix units are busy 33% of the
+// time, vector 38%, LDS 26%.  2048 tokens of 32 heads: 53 us, 650 TFLOP/s of what
+// causality leaves, 6 of them until a tile's first step is done; 8192: 890.  Two
+// buffers in turn, 8 waves, 128 keys a step, wave priorities and other orders of
+// the instructions measured no less.
 #include <type_traits>
 
 #include "kv4_attention.h"
