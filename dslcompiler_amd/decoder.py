@@ -244,9 +244,11 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
 
     q_heads is a multiple of the cache's heads; scale defaults to head_dim **
     -0.5.  The query at position p sees key j if j <= p and, with a window, j >
-    p - window or j < sinks; one that sees none gives zeros.  max_len, if the
-    caller knows it, is at least the longest of lens: the launch is planned by
-    it (by the table's size otherwise), and any value gives right results."""
+    p - window or j < sinks; one that sees none gives zeros.  Rows outside every
+    sequence (padding of a captured step) are not written: what `out` held, or
+    nothing defined.  max_len, if the caller knows it, is at least the longest
+    of lens: the launch is planned by it (by the table's size otherwise), and
+    any value gives right results."""
     dev = _begin()
     args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev)
     if out is None:

@@ -339,6 +339,20 @@ def test_rows_that_see_nothing(llk, gpu):
     assert (_bits(got) == 0).all()
 
 
+@pytest.mark.parametrize("news", [[1, 3, 2], [20, 0, 30], [130, 140]])
+def test_rows_outside_every_sequence_are_not_written(llk, gpu, news):
+    c = Case(gpu, [n + 40 for n in news], news, 2, 64, 16, seed=sum(news))
+    q = c.queries(2)
+    want, mag = ref.attention(q, c.pool, c.table, c.lens, c.starts, 64 ** -0.5)
+    pool, table, lens, starts = c.dev()
+    padded = gpu.full((c.tokens + 3, 2, 64), float("nan"), dtype=gpu.bfloat16, device="cuda")
+    padded[1:-2] = _dev(gpu, q)
+    out = gpu.full_like(padded, 5.0)
+    llk.kv4_attention(padded, pool, table, lens, starts=starts + 1, out=out)
+    check(out[1:-2], want, mag)
+    assert bool((out[:1] == 5).all()) and bool((out[-2:] == 5).all())
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_unseen_keys_never_reach_a_row(llk, gpu, D):
     """NaN keys and values past the end, after a row's position, outside its
