@@ -18,7 +18,8 @@ constexpr float kNegInf = -__builtin_inff();
 struct RowTile {
   int s, row0, rows;     // sequence; first row of the sequence; rows in it
   int first, token0;     // position and index of the sequence's first new token
-  int p_lo, p_hi;        // positions of the tile's first and last query
+  int p_lo, p_last;      // positions of the tile's first and last query
+  int p_hi;              // the last of them that the sequence holds: no later key is read
   int sink, low, steps;  // steps over the first tokens; first other step; all steps
 };
 
@@ -53,10 +54,13 @@ __device__ __forceinline__ bool row_tile(const Kv4AttentionArgs& a, int t, RowTi
   o->rows = (int)min((int64_t)R, all - row0);
   o->token0 = first;
   const int len = kv4_length(a.cache, b, o->s);
-  // new tokens past the table's end see all it holds
-  o->first = max(min(b.lens[o->s], kKv4MaxLength) - (next - first), -kKv4MaxLength);
+  // A new token past what the table holds keeps its position, of which causality
+  // and the window go; the keys there are absent.  (len, if lens is beyond the
+  // table, is whole pages, so no 16 keys that are read lie partly past it.)
+  o->first = (int)max((int64_t)b.lens[o->s] - (next - first), -(int64_t)kKv4MaxLength);
   o->p_lo = o->first + o->row0 / a.group;
-  o->p_hi = min(o->first + (o->row0 + o->rows - 1) / a.group, len - 1);
+  o->p_last = o->first + (o->row0 + o->rows - 1) / a.group;
+  o->p_hi = min(o->p_last, len - 1);
   o->sink = o->low = o->steps = 0;
   if (o->p_hi < 0) return true;
   constexpr int kStep = kv4_step(R);

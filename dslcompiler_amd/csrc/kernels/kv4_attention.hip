@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kWaves * 64)
     const int r = x * 16 + col;
     const int row = rt.row0 + (r < rt.rows ? r : 0);
     const int i = row / a.group, h = head * a.group + row % a.group;
-    pos[x] = min(rt.first + i, rt.p_hi);
+    pos[x] = rt.first + i;
     const uint16_t* src = a.q + (int64_t)(rt.token0 + i) * a.q_token + (int64_t)h * a.q_head;
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kWaves * 64)
     const int k0 = key0(step);
     // every row sees every key of the step
     const bool whole = k0 + kStep - 1 <= rt.p_lo && cur[0].present && cur[1].present &&
-                       (!a.window || k0 > rt.p_hi - a.window || k0 + kStep <= a.sinks);
+                       (!a.window || k0 > rt.p_last - a.window || k0 + kStep <= a.sinks);
     // V to LDS.  A value of a key that some row does not see must not reach
     // that row even as 0 * NaN: positions past the tile's last read as finite
     // (a scale of 0), and NaN blocks go in as zeros and are added to the rows

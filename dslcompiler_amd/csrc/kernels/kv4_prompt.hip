@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kTiles * 64)
   {
     const int r = wave * 32 + lrow, row = rt.row0 + (r < rt.rows ? r : 0);
     const int token = row / a.group, qhead = head * a.group + row % a.group;
-    pos = min(rt.first + token, rt.p_hi);
+    pos = rt.first + token;
     const uint16_t* src =
         a.q + (int64_t)(rt.token0 + token) * a.q_token + (int64_t)qhead * a.q_head + half * 8;
 #pragma unroll
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kTiles * 64)
   // positions of the wave's first and last row
   const int last = max(min(wave * 32 + 32, rt.rows) - 1, 0);
   const int w_lo = rt.first + (rt.row0 + min(wave * 32, last)) / a.group;
-  const int w_hi = min(rt.first + (rt.row0 + last) / a.group, rt.p_hi);
+  const int w_hi = rt.first + (rt.row0 + last) / a.group;
 
   f32x16 o[kD32];
   float m = kNegInf, l = 0.0f;

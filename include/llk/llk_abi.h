@@ -348,7 +348,10 @@ int64_t llk_kv4_head_bytes(int64_t page_size, int64_t head_dim);
  * page table[s * table_stride + p / page_size]; its last starts[s + 1] -
  * starts[s] positions are the call's new tokens starts[s] on.  table, lens and
  * starts are device memory and are read by the kernels, which take a position
- * past the table or on a page outside [0, pages) as absent. */
+ * past the table, from 2^30 on or on a page outside [0, pages) as absent.  A
+ * length beyond what the table holds moves no token: its last positions, the
+ * new tokens' among them, are absent, and a new token there asks (and its window
+ * ends) at its own position. */
 typedef struct llk_kv4_batch {
   const int32_t* table; /* [sequences, table_pages] */
   int64_t table_stride;
