@@ -213,6 +213,12 @@ __device__ void add_nan(const Kv4AttentionArgs& a, uint64_t flags, int c, int ke
   }
 }
 
+// An output of a row whose weights' sum is l (inv: 1 / l).  l is 0 if the row saw
+// no key, or only scores of -infinity: then zero, whatever o holds (add_nan's NaN).
+__device__ __forceinline__ float result(float o, float l, float inv) {
+  return l == 0.0f ? 0.0f : o * inv;
+}
+
 // Parts of a row's softmax (maximum m of the unscaled scores, sum l, 4 of the
 // unnormalised outputs) joined into one; m is the largest of theirs.
 struct Joined {
@@ -225,15 +231,15 @@ struct Joined {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(f, po[i], o[i]);
   }
-  // Elements d..d + 3 of the tile's row r; zeros for a row that saw no key.
+  // Elements d..d + 3 of the tile's row r.
   __device__ __forceinline__ void store(const Kv4AttentionArgs& a, const RowTile& rt, int head,
                                         int r, int d) const {
     const int row = rt.row0 + r;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     uint16_t* dst = a.out + (int64_t)(rt.token0 + row / a.group) * a.out_token +
                     (int64_t)(head * a.group + row % a.group) * a.out_head + d;
-    store8_any(dst, make_uint2(f32x2_to_bf16x2_rne(o[0] * inv, o[1] * inv),
-                               f32x2_to_bf16x2_rne(o[2] * inv, o[3] * inv)));
+    store8_any(dst, make_uint2(f32x2_to_bf16x2_rne(result(o[0], l, inv), result(o[1], l, inv)),
+                               f32x2_to_bf16x2_rne(result(o[2], l, inv), result(o[3], l, inv))));
   }
 };
 

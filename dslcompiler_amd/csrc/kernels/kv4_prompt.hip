@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kTiles * 64)
         *reinterpret_cast<f32x4*>(part + r * D + d * 32 + e * 8 + 4 * half) =
             f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
   } else {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     uint16_t* const dst = a.out + (int64_t)(rt.token0 + token) * a.out_token +
                           (int64_t)qhead * a.out_head + 4 * half;
 #pragma unroll
@@ -293,8 +293,9 @@ __global__ void __launch_bounds__(kTiles * 64)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         store8_any(dst + d * 32 + e * 8,
-                   make_uint2(f32x2_to_bf16x2_rne(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
-                              f32x2_to_bf16x2_rne(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)));
+                   make_uint2(f32x2_to_bf16x2_rne(result(o[d][4 * e], l, inv), result(o[d][4 * e + 1], l, inv)),
+                              f32x2_to_bf16x2_rne(result(o[d][4 * e + 2], l, inv),
+                                                  result(o[d][4 * e + 3], l, inv))));
   }
 }
 

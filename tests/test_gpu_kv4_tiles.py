@@ -70,3 +70,24 @@ def test_lengths_below_zero(llk, gpu, rows, news, group):
         got, want, mag = attend(llk, c, q, window=window, sinks=sinks)
         assert (want[:news[0]] == 0).all() and (want[-news[3]:] == 0).all()
         check(got, want, mag, (window, sinks))
+
+
+# ---- rows whose every score is -infinity ----------------------------------------
+
+
+@pytest.mark.parametrize("before", [20, 2500])
+@pytest.mark.parametrize("rows,news,group", [(16, [1, 1], 4), (16, [2, 3], 5), (32, [9, 8], 3),
+                                             (128, [65, 80], 2)])
+def test_scores_of_minus_infinity(llk, gpu, rows, news, group, before):
+    """Zeros, also where a value that the row sees is NaN; NaN for the other rows."""
+    c = Case(gpu, [before + n for n in news], news, 1, 64, 16, seed=rows)
+    codes, scales = ref._views(c.pool, 64)
+    keys = codes[:, :, :, 0, 0, :, 0]
+    keys[:] = keys & 0xf0 | 2  # the first element of every key: 1 times its scale
+    scales[c.table[0, 0], 0, 0, 1, 1, 5] = 255  # a block of the value at position 5
+    q = c.queries(group)
+    q[:, 0, 0] = -np.inf
+    assert (planned(llk, c, q, rows)["splits"] > 1) == (before > 1000)
+    got, want, mag = attend(llk, c, q)
+    assert (want[:, 0] == 0).all() and np.isnan(want[:news[0], 1:, 32:]).all()
+    check(got, want, mag)
