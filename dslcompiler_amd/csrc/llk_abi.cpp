@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <tuple>
 #include <atomic>
+#include <condition_variable>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -109,7 +110,7 @@ struct Workspace {
   void* ptr = nullptr;
   size_t bytes = 0;
   bool pinned = false;        // used under graph capture: a graph may name it, never freed
-  int busy = 0;               // calls between get_workspace and release_workspace
+  bool busy = false;          // a call is between get_workspace and release_workspace
   uint64_t tick = 0;          // last use, for LRU eviction
 };
 
@@ -122,6 +123,7 @@ struct DeviceState {
   // one per thread), so launches on different streams never share one; at
   // most max_workspaces of them, least recently used evicted first.
   std::map<std::pair<uintptr_t, uint64_t>, Workspace> ws;
+  std::condition_variable given_back;  // a workspace of `ws` is no longer busy
   uint64_t tick = 0;
   std::vector<void*> retired;  // outgrown pinned workspaces, kept until process exit
   void* noalloc_scratch = nullptr;  // device address of `scratch` (below)
@@ -219,7 +221,7 @@ bool evict_one_workspace(DeviceState& st, const Workspace* keep) {
   auto victim = st.ws.end();
   for (auto it = st.ws.begin(); it != st.ws.end(); ++it) {
     const Workspace& w = it->second;
-    if (&w == keep || w.busy > 0 || w.pinned) continue;
+    if (&w == keep || w.busy || w.pinned) continue;
     if (victim == st.ws.end() || w.tick < victim->second.tick) victim = it;
   }
   if (victim == st.ws.end()) return false;
@@ -233,8 +235,11 @@ bool evict_one_workspace(DeviceState& st, const Workspace* keep) {
 
 // Workspace: the caller's (ctx->scratch) if given, else the library's own
 // buffer for the launch stream, grown on demand.  Launches are ordered on
-// their stream, so work on one stream never overlaps in its workspace, and
-// two streams never share one.  (A HIP graph captured on a stream keeps
+// their stream, and a call that finds another thread's between get_workspace and
+// release_workspace waits until that one's launches are all enqueued (a main
+// kernel and the one that joins its partial results belong together), so work on
+// one stream never overlaps in its workspace, and two streams never share one.
+// (A HIP graph captured on a stream keeps
 // that stream's workspace: replaying it concurrently with direct launches
 // on the capture stream is the caller's race, as with any captured buffer.)
 // The library keeps at most `max_workspaces` of them per device (tunable,
@@ -267,9 +272,14 @@ int get_workspace(int dev, size_t need, size_t asked, llk_kernel_context* ctx, v
   if (need == 0) return LLK_OK;
   DeviceState& st = g_dev[dev];
   const auto key = workspace_key(ctx ? static_cast<hipStream_t>(ctx->stream) : nullptr);
-  std::lock_guard<std::mutex> lk(st.mu);
+  std::unique_lock<std::mutex> lk(st.mu);
   Workspace* w = nullptr;
-  if (st.ws.find(key) == st.ws.end()) {
+  auto at = st.ws.find(key);
+  while (at != st.ws.end() && at->second.busy) {
+    st.given_back.wait(lk);
+    at = st.ws.find(key);  // it may have been evicted meanwhile
+  }
+  if (at == st.ws.end()) {
     const size_t cap = (size_t)std::max<int64_t>(1, llk::tunable(llk::Knob::max_workspaces));
     while (st.ws.size() >= cap && evict_one_workspace(st, nullptr)) {
     }
@@ -282,10 +292,10 @@ int get_workspace(int dev, size_t need, size_t asked, llk_kernel_context* ctx, v
   if (w->bytes < need) {
     const size_t bytes = std::max({need, w->bytes + w->bytes / 2, (size_t)1 << 20});
     if (w->ptr) {
-      if (w->pinned || w->busy > 0 || hipFree(w->ptr) != hipSuccess) {
+      if (w->pinned || hipFree(w->ptr) != hipSuccess) {
         (void)hipGetLastError();
         try {
-          st.retired.push_back(w->ptr);  // a graph or a concurrent call may still name it
+          st.retired.push_back(w->ptr);  // a graph may still name it
         } catch (const std::bad_alloc&) {
           return fail(LLK_ERR_OUT_OF_MEMORY, "workspace bookkeeping");
         }
@@ -308,7 +318,7 @@ int get_workspace(int dev, size_t need, size_t asked, llk_kernel_context* ctx, v
     w->bytes = bytes;
     w->pinned = false;
   }
-  ++w->busy;
+  w->busy = true;
   w->tick = ++st.tick;
   *out = w->ptr;
   *held = w;
@@ -322,9 +332,12 @@ void release_workspace(int dev, Workspace* w, hipStream_t s) {
   if (!w) return;
   const bool pin = capturing(s);
   DeviceState& st = g_dev[dev];
-  std::lock_guard<std::mutex> lk(st.mu);
-  if (pin) w->pinned = true;
-  --w->busy;
+  {
+    std::lock_guard<std::mutex> lk(st.mu);
+    if (pin) w->pinned = true;
+    w->busy = false;
+  }
+  st.given_back.notify_all();
 }
 
 // Workspace of llk_swiglu_bf16_noalloc: a fixed device array, one copy per
