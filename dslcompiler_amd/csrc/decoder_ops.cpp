@@ -157,6 +157,9 @@ int check_move(const llk_tensor3d* k, const llk_tensor3d* v, const llk_kv4_cache
   if ((rc = check_rows3(k, "k", b->tokens, c->heads, cache->head_dim, result)) ||
       (rc = check_rows3(v, "v", b->tokens, c->heads, cache->head_dim, result)))
     return rc;
+  if (b->tokens > kKv4MaxMoved)
+    return fail(LLK_ERR_SHAPE, "%d tokens are too many for one call (%lld)", b->tokens,
+                (long long)kKv4MaxMoved);
   *r = Kv4Rows{bf16_of(k), bf16_of(v), k->stride0, k->stride1, v->stride0, v->stride1};
   // (a read without sequences gives zeros)
   *empty = b->tokens == 0 || (b->sequences == 0 && !result);
@@ -253,9 +256,9 @@ int check_attention(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk
                 (long long)batch->tokens, a->group);
   *plan = plan_attention(a->batch, a->cache.page_shift, a->cache.heads, a->group,
                          (int)cache->head_dim, a->window, a->sinks, batch->max_len);
-  if (plan->tiles * heads > 0x7fffffff)
-    return fail(LLK_ERR_SHAPE, "%lld row tiles of %lld heads are too many", (long long)plan->tiles,
-                (long long)heads);
+  if (plan->tiles * heads > kKv4MaxWorkgroups)
+    return fail(LLK_ERR_SHAPE, "%lld row tiles of %lld heads are too many for one call (%lld)",
+                (long long)plan->tiles, (long long)heads, (long long)kKv4MaxWorkgroups);
   a->tiles = (int)plan->tiles;
   a->splits = plan->splits;
   a->chunk = plan->chunk;
@@ -272,7 +275,7 @@ int llk_block_norm(const llk_tensor2d* y, const llk_tensor2d* residual, llk_tens
     return fail(LLK_ERR_INVALID_ARGUMENT, "%s is NULL",
                 !residual ? "residual" : !out ? "out" : "params");
   const int64_t M = residual->dim0, N = residual->dim1;
-  if (M < 0 || N < 1 || N > kBlockNormMaxN || M > 0x7fffffff)
+  if (M < 0 || N < 1 || N > kBlockNormMaxN)
     return fail(LLK_ERR_SHAPE, "residual of (%lld, %lld) unsupported (1 to %lld columns)",
                 (long long)M, (long long)N, (long long)kBlockNormMaxN);
   int rc;

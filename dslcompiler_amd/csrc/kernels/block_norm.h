@@ -17,7 +17,7 @@ struct BlockNormArgs {
 // Largest N: 1024 threads of 4 chunks of 8 elements.
 constexpr int64_t kBlockNormMaxN = 32768;
 
-// 1 <= M < 2^31, 1 <= N <= kBlockNormMaxN; *_f32: fp32 instead of bf16 (y and
+// M >= 1 (in as many launches as its threads need), 1 <= N <= kBlockNormMaxN; *_f32: fp32 instead of bf16 (y and
 // the gate; the residual, in and out; the result; both weights).
 hipError_t llk_launch_block_norm(const BlockNormArgs& a, int64_t M, bool y_f32, bool h_f32,
                                  bool o_f32, bool w_f32, hipStream_t s);

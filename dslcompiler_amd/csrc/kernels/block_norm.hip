@@ -13,6 +13,8 @@
 // the unrounded sum.
 #include "block_norm.h"
 
+#include <algorithm>
+
 #include "common.h"
 
 namespace llk_gfx950 {
@@ -191,5 +193,20 @@ hipError_t llk_launch_block_norm(const BlockNormArgs& a, int64_t M, bool y_f32, 
                              : pick<4>(y_f32, h_f32, o_f32, w_f32);
   BlockNormArgs args = a;
   void* params[] = {&args};
-  return hipLaunchKernel(fn, dim3((unsigned)M), dim3(threads), params, 0, s);
+  // a dimension of a launch takes fewer than 2^32 threads; with more it runs some
+  // of them only, and says nothing
+  const int64_t most = ((int64_t)1 << 31) / threads;
+  auto advance = [&](const void*& p, int64_t ld, bool f32) {
+    if (p) p = static_cast<const uint8_t*>(p) + most * ld * (f32 ? 4 : 2);
+  };
+  for (int64_t left = M;; left -= most) {
+    const hipError_t e =
+        hipLaunchKernel(fn, dim3((unsigned)std::min(left, most)), dim3(threads), params, 0, s);
+    if (e != hipSuccess || left <= most) return e;
+    advance(args.y, a.ldy, y_f32);
+    advance(args.g, a.ldg, y_f32);
+    advance(args.h, a.ldh, h_f32);
+    if (args.h_out) args.h_out = static_cast<uint8_t*>(args.h_out) + most * a.ldho * (h_f32 ? 4 : 2);
+    args.out = static_cast<uint8_t*>(args.out) + most * a.ldo * (o_f32 ? 4 : 2);
+  }
 }

@@ -56,6 +56,12 @@ struct Kv4AttentionArgs {
   float scale;        // of q.k, times log2(e)
 };
 
+// A dimension of a launch takes fewer than 2^32 threads (with more it runs some of
+// them only): workgroups of 256, and tokens at 16 to a workgroup of the write and
+// the read.
+constexpr int64_t kKv4MaxWorkgroups = ((int64_t)1 << 24) - 1;
+constexpr int64_t kKv4MaxMoved = kKv4MaxWorkgroups * 16;
+
 // k, v (out for read): element strides of tokens and heads.
 struct Kv4Rows {
   uint16_t *k, *v;

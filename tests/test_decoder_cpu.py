@@ -200,3 +200,26 @@ def test_python_refusals(llk):
         llk.kv4_cache(4, 2, 48, 128, device="cpu")
     cache = llk.kv4_cache(4, 2, 64, 128, device="cpu")
     assert cache.shape == (4, 2, 4 * 17 * 128) and cache.dtype == torch.uint8
+
+
+def test_sizes_beyond_one_launch(L):
+    """A dimension of a launch takes fewer than 2^32 threads: 2^24 - 1 workgroups of
+    256; what needs more is refused by its size, before any device work."""
+    from dslcompiler_amd._lib import AttentionPlan
+    plan, n = AttentionPlan(), 1 << 23
+
+    def describe(sequences):
+        return L.llk_kv4_attention_describe(_kv(T=sequences, H=8), _cache(),
+                                            _batch(sequences=sequences, tokens=sequences), _par(),
+                                            plan)
+
+    assert describe(n - 1) == 0 and plan.workgroups == 2 * (n - 1)  # 2 key heads
+    assert describe(n) == -2 and b"too many" in L.llk_last_error()
+    q = _kv(T=n, H=8)
+    assert L.llk_kv4_attention(q, _cache(), _batch(sequences=n, tokens=n), _par(), q, None) == -2
+    most = ((1 << 24) - 1) * 16  # tokens written or read, 16 to a workgroup
+    k = _kv(T=most + 1)
+    b = _batch(sequences=1, tokens=most + 1, starts=FAKE)
+    assert L.llk_kv4_write(k, k, _cache(), b, None) == -2
+    assert L.llk_kv4_read(_cache(), b, k, k, None) == -2
+    assert str(most).encode() in L.llk_last_error()

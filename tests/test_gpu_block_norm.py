@@ -184,3 +184,20 @@ def test_stream_and_graph(llk, gpu):
         gpu.cuda.synchronize()
         for a, b in zip(want, out):
             assert gpu.equal(a, b), k
+
+
+def test_rows_beyond_one_launch(llk, gpu):
+    """2^26 rows and more of narrow ones: 2^32 threads at a wave to a row, more
+    than a dimension of one launch takes."""
+    M, N = (1 << 26) + 3, 2
+    h = gpu.zeros((M, N), dtype=gpu.bfloat16, device="cuda")
+    at = [0, 1, (1 << 24) - 1, 1 << 24, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, M - 1]
+    for i, m in enumerate(at):
+        h[m, 0], h[m, 1] = 1 + i, -0.5 * i
+    w = gpu.tensor([1.0, 2.0], device="cuda").bfloat16()
+    y = h * 2
+    r, n = llk.block_norm(y, h, w)
+    want_r, want_n, mr, mn = reference(y[at], h[at], w)
+    close(r[at], want_r, mr, "residual")
+    close(n[at], want_n, mn, "out")
+    assert int((r != 0).sum()) == int((h != 0).sum()) == int((n != 0).sum())
