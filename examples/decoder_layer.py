@@ -103,9 +103,9 @@ def main() -> None:
 
     replay = step
     if a.graph:
-        side = torch.cuda.Stream()
-        side.wait_stream(torch.cuda.current_stream())
         held = token.clone(), lens.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())  # for what the step changes, copied above
         with torch.cuda.stream(side):  # the library's workspace of this stream
             step()
         torch.cuda.synchronize()
@@ -123,7 +123,7 @@ def main() -> None:
     end.record()
     torch.cuda.synchronize()
     print(f"{a.layers} layers, prompts {prompts}, {a.tokens} tokens: lengths {lens.tolist()}, "
-          f"rms {token.float().square().mean().sqrt().item():.4f}, "
+          f"last token begins {[round(v, 4) for v in token[:, :3].flatten().tolist()]}, "
           f"{begin.elapsed_time(end) / a.tokens * 1e3:.1f} us a step")
 
 

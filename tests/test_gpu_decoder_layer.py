@@ -112,3 +112,16 @@ def test_runs_as_a_program():
         assert r.returncode == 0, r.stdout + r.stderr
         assert "lengths [63, 23]" in r.stdout
         assert "nan" not in r.stdout
+
+
+def test_program_gives_the_same_with_a_graph():
+    """Lengths and the last token after the same steps, eager and replayed
+    (the step before the capture changes both, from which they are restored)."""
+    said = []
+    for more in ([], ["--graph"]):
+        r = subprocess.run([sys.executable, str(ROOT / "examples" / "decoder_layer.py"),
+                            "--prompt", "300", "--tokens", "5", *more],
+                           capture_output=True, text=True, timeout=100)
+        assert r.returncode == 0, r.stdout + r.stderr
+        said.append(r.stdout.split("us a step")[0].rsplit(",", 1)[0])
+    assert said[0] == said[1] and "lengths [305, 105]" in said[0]
