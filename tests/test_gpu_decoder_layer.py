@@ -125,3 +125,62 @@ def test_program_gives_the_same_with_a_graph():
         assert r.returncode == 0, r.stdout + r.stderr
         said.append(r.stdout.split("us a step")[0].rsplit(",", 1)[0])
     assert said[0] == said[1] and "lengths [305, 105]" in said[0]
+
+
+def test_captured_steps(llk, gpu, monkeypatch):
+    """A decoded token's step captured once: each replay, with new lengths and
+    tokens, equals the eager step bit by bit and the layers in 64 bits."""
+    model, mats = make(gpu, monkeypatch, hidden=256, inner=512, heads=4, kv_heads=2, head_dim=64,
+                       pages=16, page_size=16, window=40, sinks=3)
+    gen = gpu.Generator(device="cuda").manual_seed(4)
+    table = gpu.randperm(16, generator=gen, device="cuda").int().view(2, 8)
+    lens = gpu.tensor([45, 60], dtype=gpu.int32, device="cuda")
+    starts = gpu.tensor([0, 45, 105], dtype=gpu.int32, device="cuda")
+    x = gpu.randn(105, 256, generator=gen, device="cuda").bfloat16()
+    model.forward(x, table, lens, starts)
+    token = gpu.randn(2, 256, generator=gen, device="cuda").bfloat16()
+    lens += 1
+    side = gpu.cuda.Stream()
+    side.wait_stream(gpu.cuda.current_stream())
+    with gpu.cuda.stream(side):
+        model.forward(token, table, lens)
+    gpu.cuda.synchronize()
+    graph = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(graph, stream=side):
+        out = model.forward(token, table, lens)
+    bound = 2 * 10 * 2.0 ** -9
+    for n in range(4):
+        graph.replay()
+        got = out.clone()
+        want = reference(model, mats, token, table.cpu().numpy(), lens.cpu().numpy(), None)
+        assert np.linalg.norm(got.double().cpu().numpy() - want) <= bound * np.linalg.norm(want), n
+        assert gpu.equal(model.forward(token, table, lens), got), n
+        token.copy_(got)
+        lens += 1
+
+
+def test_token_by_token_against_the_prompt_at_once(llk, gpu, monkeypatch):
+    """The same 75 tokens through pages of their own.
+
+    Bound.  Each pass is within b = 20 * 2^-9 of the layers over its own cache, and
+    the caches differ where a code comes out otherwise.  Layer 1 quantises the same
+    keys and values but for rare roundings.  Those of layer 2 differ by at most b / 2
+    of their size; a code's step is at most 0.63 of a block's rms (the scale is at
+    most 2 / 7 of the largest of 32, about 2.2 rms, and steps are 1 or less below 4),
+    so the quantised ones by sqrt(0.63 * b / 2) = 0.11 of it, and attention by as much
+    through the values and as much through the scores: 0.16.  With the layer's weight
+    of 1/2 in the residual, twice (attention, and the MLP behind it): 0.16 * 0.5 *
+    sqrt(2) = 0.11.  In all 2 b + 0.11 < 0.19."""
+    model, _ = make(gpu, monkeypatch, hidden=256, inner=512, heads=4, kv_heads=2, head_dim=64,
+                    pages=16, page_size=16, window=40, sinks=3)
+    gen = gpu.Generator(device="cuda").manual_seed(6)
+    n = 75
+    x = gpu.randn(n, 256, generator=gen, device="cuda").bfloat16()
+    table = gpu.randperm(16, generator=gen, device="cuda").int().view(2, 8)
+    starts = gpu.tensor([0, n], dtype=gpu.int32, device="cuda")
+    lens = gpu.tensor([n], dtype=gpu.int32, device="cuda")
+    whole = model.forward(x, table[:1], lens, starts).double()
+    for i in range(n):
+        lens.fill_(i + 1)
+        got = model.forward(x[i:i + 1], table[1:], lens).double()
+        assert (got - whole[i]).norm() <= 0.19 * whole[i].norm(), i
