@@ -13,6 +13,7 @@ from .ops import (PackedWeights, classify_m, describe_launch, device_info,  # no
                   workspace_stats, workspace_trim)
 
 __all__ = ["JitCache", "KernelKey", "LLKError", "PackedWeights", "WeightKey", "block_norm",
-           "classify_m", "describe_kv4_attention", "describe_launch", "device_info", "fill_normal_bf16", "fused_swiglu", "get_tunable",
-           "kv4_attention", "kv4_cache", "kv4_read", "kv4_write", "lib", "matmul", "mlp", "pack_device_layout", "select_schedule", "set_schedule_db",
-           "set_tunable", "swiglu_scratch_size", "workspace_stats", "workspace_trim"]
+           "classify_m", "describe_kv4_attention", "describe_launch", "device_info",
+           "fill_normal_bf16", "fused_swiglu", "get_tunable", "kv4_attention", "kv4_cache",
+           "kv4_read", "kv4_write", "lib", "matmul", "mlp", "pack_device_layout",
+           "select_schedule", "set_schedule_db", "set_tunable", "swiglu_scratch_size", "workspace_stats", "workspace_trim"]

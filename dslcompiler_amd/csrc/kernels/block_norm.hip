@@ -8,7 +8,9 @@
 //
 // HBM bound: y, h and g are read once and h', n written once, since a row stays
 // in registers between the two sums (a workgroup per row, CH chunks of 8
-// elements per thread).  All arithmetic and both sums are in fp32; h' is
+// elements per thread; with 4 chunks, above 16384 columns, part of it spills unless
+// y and the weights are bf16: 4097 rows of fp32 with a gate, 16384 columns 268 us,
+// 5.0 TB/s, 32768 columns 688 us, 3.9; of bf16 127 us, 5.3, and 290 us, 4.6).  All arithmetic and both sums are in fp32; h' is
 // rounded to the residual's type only where it is stored, so n is the norm of
 // the unrounded sum.
 #include "block_norm.h"
@@ -182,9 +184,12 @@ hipError_t llk_launch_block_norm(const BlockNormArgs& a, int64_t M, bool y_f32, 
                                  bool o_f32, bool w_f32, hipStream_t s) {
   using namespace llk_gfx950;
   const int chunks = (a.N + 7) / 8;
-  // Chunks to a thread: one where few rows leave CUs idle (17 x 5120: 6.3 us,
-  // with two 6.9), two where there are enough (4097 x 5120 with a gate, bf16: 47
-  // us, with one 54); more only where 1024 threads are too few.
+  // Chunks to a thread: one where few rows leave CUs idle, two where there are
+  // enough; more only where 1024 threads are too few.  Bf16 rows of 5120 with a gate,
+  // one and two chunks, us: 17 rows 6.3 and 6.7, 256 6.8 and 7.2, 512 10.0 both, 640
+  // 12.2 and 11.2, 1024 15.0 and 13.6, 4097 50 and 41.  (fp32 rows of 4096 without
+  // one do better with one chunk at any number: 1024 rows 13.3 and 13.8, 4097 41 and
+  // 45.)
   int ch = M <= 512 ? 1 : 2;
   while (chunks > ch * 1024) ch *= 2;
   const int threads = ((chunks + ch - 1) / ch + 63) / 64 * 64;

@@ -25,16 +25,21 @@ namespace {
 constexpr int kWaves = 4;  // of a workgroup, each over its own keys
 constexpr int kStep = 32;  // keys to a step
 
-// Waves to a SIMD that the registers are cut to: more bytes on their way (D =
-// 128, one row tile: 4 instead of 3, one token over 131072 keys 34.8 -> 30.7 us).
+// Waves to a SIMD that the registers are cut to: more have more bytes on their way
+// until the registers no longer suffice.  D = 128, 16 rows: one token over 131072
+// keys, 3 waves 34.8 us, 4 30.7.  Ragged sequences to 8192 keys (D = 256: 4096), 64
+// with 16 rows, 32 with 32 rows, us: D = 64, 16 rows, 4 waves 52, 5 51.7, 6 49.5; 32
+// rows, 3 waves 41, 5 88; D = 128, 16 rows, 3 to 5 waves 77; 32 rows, 1 wave 100, 2
+// 65, 3 86; D = 256, 16 rows, 1 wave 113, 2 82, 3 112; 32 rows, 1 wave 113, 2 207.
 template <int D, int RT>
-constexpr int kMinWaves = D * RT <= 64 ? 5 : D * RT <= 128 ? (RT == 1 ? 4 : 3) : D * RT <= 256 ? 2 : 1;
+constexpr int kMinWaves =
+    D * RT <= 64 ? 5 : D * RT <= 128 ? (RT == 1 ? 4 : 3) : D * RT <= 256 ? 2 : 1;
 
 // A workgroup's 4 waves share a row tile of 16 * RT rows and one split of its
 // keys, each wave taking every fourth step of 32 keys with a running maximum
 // of its own; at the end they are joined in LDS.
 // Bound by HBM for 16 rows: 64 sequences of 4.2k keys on average (358 MB) take
-// 69 us, 5.2 TB/s; one token over 131072 keys (143 MB) 28 us, 5.1 TB/s, and 4 to
+// 68 us, 5.3 TB/s; one token over 131072 keys (143 MB) 28 us, 5.1 TB/s, and 4 to
 // join the splits.  The codes of one row tile are read past the L2, since no
 // other workgroup reads them.
 template <int D, int RT>
@@ -243,7 +248,8 @@ __global__ void __launch_bounds__(kWaves * 64)
   for (int y = 0; y < RT; ++y) l[y] = sum_over_groups(l[y]);
   if (grp == 0) {
 #pragma unroll
-    for (int y = 0; y < RT; ++y) wave_m[wave][y * 16 + col] = m[y], wave_l[wave][y * 16 + col] = l[y];
+    for (int y = 0; y < RT; ++y)
+      wave_m[wave][y * 16 + col] = m[y], wave_l[wave][y * 16 + col] = l[y];
   }
   float* const part = used > 1 ? part_of<D, R>(a, tile, head, split) : nullptr;
   // 16 rows at a time fit the waves' own V buffers (32 keys x 2 bytes = 16
@@ -277,9 +283,11 @@ __global__ void __launch_bounds__(kWaves * 64)
   }
 }
 
-// Up to so many splits a row is joined by one group of threads (4 splits of 64
-// sequences, 4 rows each: 4.6 us, by a workgroup to a row 5.8; 2 of 1000 tokens of
-// 32 heads: the call 38 us, 72), more by a workgroup (64 splits: 22 us, 27).
+// Up to so many splits a row is joined by one group of threads, more by a workgroup
+// to a row.  The call by the one and the other, us: 32 rows, 4 splits 9.3 and 9.8, 8
+// 10.2 both, 16 10.9 and 10.4, 64 17.4 and 13.0; 256 rows, 4 splits 10.4 and 10.6, 8
+// 12.7 and 12.6, 12 14.0 and 13.7, 32 24.9 and 23.2; 2048 rows, 8 splits 16.5 and
+// 18.7, 12 21.8 and 23.8, 16 26.9 and 27.4; 6400 rows, 8 splits 25 and 32.
 constexpr int kJoinAlone = 8;
 
 // Joins the splits of a row in their order.  A group of D / 4 threads takes 4 of

@@ -180,8 +180,11 @@ template <int D>
 hipError_t write(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, hipStream_t s) {
   return launch_rows(&kv4_write_kernel<D>, c, b, r, D, s);
 }
-// From 64 MiB of keys and values on they are written past the L2: 43530 tokens
-// of 8 heads of 128 (178 MB) 82 -> 52 us, 2048 tokens of 32 (34 MB) 10.9 -> 12.1.
+// From 64 MiB of keys and values on they are written past the L2.  8 heads of 128,
+// through the L2 and past it, us, into memory other than the last call's: 50 MB 14.2
+// and 16.6, 67 MB 24 and 21, 101 MB 38 and 29, 134 MB 57 and 39, 178 MB 76 and 52, 268
+// MB 113 and 78.  (Into the same memory again and again, as a replayed graph does, the
+// caches hold it for longer: 67 MB 17.5 and 21, 134 MB 30 and 39, 147 MB 47 and 44.)
 template <int D>
 hipError_t read(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, hipStream_t s) {
   const bool past = (int64_t)b.tokens * c.heads * D * 4 >= (int64_t)64 << 20;

@@ -7,13 +7,16 @@
 // where all four read them as operands, while the next step's codes are on their
 // way.
 //
-// Bound by no one unit: at D = 128 a workgroup alone takes ~3500 clocks (1.7 us) a
-// step, of which its matrix instructions are 1024, and two on a CU, which is what
-// the registers leave room for, ~2100 each.  Matrix units are busy 33% of the
-// time, vector 38%, LDS 26%.  2048 tokens of 32 heads: 53 us, 650 TFLOP/s of what
-// causality leaves, 6 of them until a tile's first step is done; 8192: 890.  Two
-// buffers in turn, 8 waves, 128 keys a step, wave priorities and other orders of
-// the instructions measured no less.
+// At D = 128 a step takes 1.4 us where a workgroup has its CU to itself and 2.1 us
+// where two share it, which is what the registers leave room for: 1.05 us a step.
+// With CUs kept full by equal tiles that is 940 TFLOP/s (2048 tokens of 32 heads
+// over 6080 keys each: 218 us).  The tiles of a causal prompt are not equal: 2048
+// tokens of 32 heads, 2 to 32 steps, take 53 us, 650 TFLOP/s of what causality
+// leaves and no less than 16 heads do, since the longest tiles run most of their
+// steps alone on their CU (6 us go by until a tile's first step is done); 8192
+// tokens, whose tiles refill the CUs, 890.  Over the prompt of 2048 matrix units are
+// busy 33% of the time, vector 38%, LDS 26%.  Two buffers in turn, 8 waves, 128 keys
+// a step, wave priorities and other orders of the instructions measured no less.
 #include <type_traits>
 
 #include "kv4_attention.h"
@@ -293,7 +296,8 @@ __global__ void __launch_bounds__(kTiles * 64)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         store8_any(dst + d * 32 + e * 8,
-                   make_uint2(f32x2_to_bf16x2_rne(result(o[d][4 * e], l, inv), result(o[d][4 * e + 1], l, inv)),
+                   make_uint2(f32x2_to_bf16x2_rne(result(o[d][4 * e], l, inv),
+                                                  result(o[d][4 * e + 1], l, inv)),
                               f32x2_to_bf16x2_rne(result(o[d][4 * e + 2], l, inv),
                                                   result(o[d][4 * e + 3], l, inv))));
   }

@@ -305,7 +305,7 @@ typedef struct llk_block_norm_params {
  * with r the sum before its rounding to residual_dtype.  All arithmetic in
  * fp32.  y NULL: r = residual (the norm before the first block); then
  * post_weight and gate must be NULL and residual_out may be.  residual_out may
- * be residual, out may be y (the same strides).  1 <= N <= 32768; rows at any
+ * be residual, out may be y (the same type and strides).  1 <= N <= 32768; rows at any
  * alignment of their elements.  M == 0 launches nothing. */
 int llk_block_norm(const llk_tensor2d* y, const llk_tensor2d* residual,
                    llk_tensor2d* residual_out, llk_tensor2d* out,
