@@ -135,6 +135,12 @@ class AttentionPlan(C.Structure):
                 ("launches", C.c_int64), ("workspace_bytes", C.c_size_t)]
 
 
+class Q4WeightsC(C.Structure):
+    """llk_q4_weights."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("K", C.c_int64),
+                ("N", C.c_int64), ("group", C.c_int64)]
+
+
 class LLKError(RuntimeError):
     """A negative llk_status, with the library's message."""
 
@@ -151,6 +157,7 @@ T3 = C.POINTER(Tensor3D)
 KC = C.POINTER(Kv4Cache)
 KB = C.POINTER(Kv4Batch)
 AP = C.POINTER(AttentionParams)
+Q4 = C.POINTER(Q4WeightsC)
 KKP = C.POINTER(KernelKeyC)
 WKP = C.POINTER(WeightKeyC)
 # llk_kernel_fn: the shape of llk_swiglu_bf16
@@ -199,6 +206,12 @@ SIGNATURES = {
     "llk_kv4_read": (C.c_int, [KC, KB, T3, T3, CTX]),
     "llk_kv4_attention": (C.c_int, [T3, KC, KB, AP, T3, CTX]),
     "llk_kv4_attention_describe": (C.c_int, [T3, KC, KB, AP, C.POINTER(AttentionPlan)]),
+    "llk_q4_code_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "llk_q4_scale_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "llk_q4_quantise": (C.c_int, [T2, C.c_int64, T2, T2, C.c_int, T2, CTX]),
+    "llk_q4_pack": (C.c_int, [T2, T2, C.c_int, T2, Q4, CTX]),
+    "llk_q4_gemm": (C.c_int, [T2, Q4, T2, C.c_int, C.c_int, CTX]),
+    "llk_q4_swiglu": (C.c_int, [T2, Q4, Q4, T2, C.c_int, CTX]),
     "llk_classify_m": (C.c_int, [C.c_int64]),
     "llk_num_tiles": (C.c_int64, [C.c_int64, C.c_int64]),
     "llk_tile_size": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64]),

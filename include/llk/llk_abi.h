@@ -410,6 +410,55 @@ int llk_kv4_attention_describe(const llk_tensor3d* q, const llk_kv4_cache* cache
                                llk_attention_plan* out);
 
 /* ----------------------------------------------------------------------- */
+/* Weights in 4 bits (no counterpart in the reference)                      */
+/* ----------------------------------------------------------------------- */
+
+/* W[k][n] = scale[k / group][n] * (code[k][n] - zero[k / group][n]), codes and
+ * zeros 0..15, in the kernels' order, in caller-owned device memory (16-byte
+ * aligned, of llk_q4_code_bytes and llk_q4_scale_bytes).  The last group is as
+ * long as K leaves it. */
+typedef struct llk_q4_weights {
+  void* codes;
+  void* scales;
+  int64_t K, N;
+  int64_t group; /* 32, 64 or 128 */
+} llk_q4_weights;
+
+/* Sizes of the two buffers (0 for an unsupported size). */
+size_t llk_q4_code_bytes(int64_t K, int64_t N);
+size_t llk_q4_scale_bytes(int64_t K, int64_t N, int64_t group);
+
+/* Weights bf16 [K, N] to codes uint8 [K, N], scales [ceil(K / group), N] of
+ * scale_dtype (LLK_BF16 or LLK_FP16) and zeros uint8 [ceil(K / group), N]; all
+ * device memory with unit inner stride.  zeros NULL: zero 8, scale = largest
+ * magnitude of the group / 7.  Otherwise scale = (largest - smallest of the
+ * group's values and 0) / 15 and the zero where 0 lies.  The scale is rounded to
+ * its type, then each value to the nearest code (ties to even), held to 0..15.
+ * A group with an infinity or a NaN gets the scale NaN; one whose scale rounds
+ * to 0 or infinity gets its zero as every code. */
+int llk_q4_quantise(const llk_tensor2d* w, int64_t group, llk_tensor2d* codes,
+                    llk_tensor2d* scales, int scale_dtype, llk_tensor2d* zeros,
+                    llk_kernel_context* ctx);
+
+/* Codes, scales and zeros (as above; the low 4 bits of codes and zeros count;
+ * zeros NULL: 8) into `out`, whose sizes and buffers the caller has set. */
+int llk_q4_pack(const llk_tensor2d* codes, const llk_tensor2d* scales, int scale_dtype,
+                const llk_tensor2d* zeros, const llk_q4_weights* out, llk_kernel_context* ctx);
+
+/* Y = X W, or Y += X W with accumulate: x bf16 [M, K] at any row stride and
+ * alignment of its elements, y [M, N] of y_dtype LLK_BF16, LLK_FP16 or LLK_FP32.
+ * Sums in fp32, and no weight is rounded.  A row of X with an infinity or a NaN,
+ * or whose magnitudes times 2 sum beyond fp32 over a group, gives NaN or infinity
+ * in its row of Y.  K == 0 gives zeros (leaves Y with accumulate). */
+int llk_q4_gemm(const llk_tensor2d* x, const llk_q4_weights* w, llk_tensor2d* y, int y_dtype,
+                int accumulate, llk_kernel_context* ctx);
+
+/* Y = SiLU(X Wg) * (X Wu) on weights of one shape and group, y_dtype LLK_BF16 or
+ * LLK_FP32; otherwise as llk_q4_gemm. */
+int llk_q4_swiglu(const llk_tensor2d* x, const llk_q4_weights* wg, const llk_q4_weights* wu,
+                  llk_tensor2d* y, int y_dtype, llk_kernel_context* ctx);
+
+/* ----------------------------------------------------------------------- */
 /* Shape specialisation and schedules                                       */
 /* ----------------------------------------------------------------------- */
 

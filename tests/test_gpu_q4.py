@@ -1,0 +1,250 @@
+"""4-bit weights with group scales against their definition in 64 bits.
+
+Exact cases: X of integers to 3 and scales of powers of two from 1/8 to 2, with
+which every product and sum is a multiple of 2^-7 below 4104 * 3 * 2 * 2 < 2^16, so
+fp32 adds without rounding: fp32 results are equal, bf16 and fp16 ones equal after
+one rounding.
+
+Bound of the others: a group's two sums have at most 128 terms of |x| (1 + c / 16)
+<= 2 |x| and are scaled by 16 s, and with the groups, the waves and the result at
+most 128 + K / 32 + 32 roundings of 2^-24 each of what has been summed:
+|error| <= (160 + K / 32) 2^-24 64 sum(s |x|) before the rounding to the result's
+type."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def case(torch, M, K, N, group, zeros, scale_dtype, seed, exact):
+    """x bf16, codes, scales, zeros on the device."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def ints(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=gen, device="cuda")
+
+    groups = -(-K // group)
+    codes = ints(0, 16, K, N).to(torch.uint8)
+    z = ints(0, 16, groups, N).to(torch.uint8) if zeros else None
+    if exact:
+        x = ints(-3, 4, M, K).to(torch.bfloat16)
+        scales = torch.exp2(ints(-3, 2, groups, N).float()).to(scale_dtype)
+    else:
+        x = torch.randn(M, K, generator=gen, device="cuda").bfloat16()
+        scales = (torch.randn(groups, N, generator=gen, device="cuda") * 0.02).to(scale_dtype)
+    return x, codes, scales, z
+
+
+def dense(codes, scales, z, group):
+    """W in float64."""
+    K = codes.shape[0]
+    rows = np.arange(K) // group
+    c = codes.cpu().numpy().astype(np.float64)
+    zero = 8.0 if z is None else z.cpu().numpy().astype(np.float64)[rows]
+    return (c - zero) * scales.double().cpu().numpy()[rows]
+
+
+def f64(t):
+    return t.double().cpu().numpy()
+
+
+def bound(x, scales, group, K):
+    rows = np.arange(K) // group
+    return (160 + K / 32) * 2.0 ** -24 * 64 * (np.abs(f64(x)) @ np.abs(f64(scales))[rows])
+
+
+STEP = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11, "float32": 2.0 ** -24}
+SIZES = [(1, 128, 16), (1, 1, 1), (1, 4104, 48), (2, 7, 17), (3, 31, 100), (4, 32, 15), (5, 33, 16),
+         (8, 64, 33), (9, 127, 16), (13, 129, 40), (16, 200, 64), (17, 1000, 72), (33, 640, 130),
+         (64, 256, 96), (65, 300, 257), (100, 2048, 64), (129, 384, 272), (300, 520, 80)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_exact_products(llk, gpu, M, K, N, group):
+    for zeros, st in ((False, gpu.bfloat16), (True, gpu.float16)):
+        x, codes, scales, z = case(gpu, M, K, N, group, zeros, st, M * K + N, True)
+        w = llk.Q4Weights.from_codes(codes, scales, z, group=group)
+        want = f64(x) @ dense(codes, scales, z, group)
+        got = llk.q4_matmul(x, w)
+        assert got.dtype == gpu.float32 and got.shape == (M, N)
+        assert np.array_equal(f64(got), want), (zeros, np.abs(f64(got) - want).max())
+        exact32 = gpu.from_numpy(want).float().cuda()
+        for t in (gpu.bfloat16, gpu.float16):
+            assert gpu.equal(llk.q4_matmul(x, w, out_dtype=t), exact32.to(t))
+        acc = gpu.full((M, N), 0.5, device="cuda")
+        assert llk.q4_matmul(x, w, out=acc, accumulate=True) is acc
+        assert np.array_equal(f64(acc), want + 0.5)
+
+
+@pytest.mark.parametrize("M,K,N,group", [(1, 4096, 512, 128), (1, 13824, 96, 32), (4, 1000, 200, 64),
+                                         (7, 5120, 130, 128), (16, 2048, 64, 32), (40, 777, 96, 64),
+                                         (130, 4096, 64, 128), (255, 1000, 300, 32)])
+def test_products(llk, gpu, M, K, N, group):
+    for zeros, st in ((False, gpu.float16), (True, gpu.bfloat16)):
+        x, codes, scales, z = case(gpu, M, K, N, group, zeros, st, K + N, False)
+        w = llk.Q4Weights.from_codes(codes, scales, z, group=group)
+        want = f64(x) @ dense(codes, scales, z, group)
+        most = bound(x, scales, group, K)
+        for t in (gpu.float32, gpu.bfloat16, gpu.float16):
+            got = f64(llk.q4_matmul(x, w, out_dtype=t))
+            step = STEP[str(t).split(".")[1]]
+            # (fp16 below its normal range: half its smallest step)
+            assert (np.abs(got - want) <= most * (1 + step) + step * np.abs(want) + 2.0 ** -25).all()
+        first = gpu.randn(M, N, device="cuda").bfloat16()
+        got = f64(llk.q4_matmul(x, w, out=first.clone(), accumulate=True))
+        total = want + f64(first)
+        assert (np.abs(got - total) <= most * 1.01 + 2.0 ** -8 * np.abs(total) + 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("M,K,N,group", [(1, 4096, 272, 128), (1, 100, 16, 32), (3, 640, 100, 64),
+                                         (8, 1000, 48, 32), (16, 512, 65, 128), (17, 5120, 96, 32),
+                                         (64, 300, 128, 128), (150, 1024, 136, 64)])
+def test_swiglu(llk, gpu, M, K, N, group):
+    for zeros in (False, True):
+        x, *g = case(gpu, M, K, N, group, zeros, gpu.bfloat16, 7 * K + N, False)
+        _, *u = case(gpu, M, K, N, group, zeros, gpu.bfloat16, 7 * K + N + 1, False)
+        x = (x.float() * 0.5).bfloat16()
+        wg, wu = (llk.Q4Weights.from_codes(*s, group=group) for s in (g, u))
+        a, b = f64(x) @ dense(*g, group), f64(x) @ dense(*u, group)
+        ea, eb = bound(x, g[1], group, K), bound(x, u[1], group, K)
+        silu = a / (1 + np.exp(-a))
+        # SiLU's slope is below 1.1; the activation itself within 4 ulp
+        most = 1.1 * ea * (np.abs(b) + eb) + np.abs(silu) * eb + 2.0 ** -21 * np.abs(silu * b)
+        for t, step in ((gpu.float32, 2.0 ** -24), (gpu.bfloat16, 2.0 ** -8)):
+            got = f64(llk.q4_swiglu(x, wg, wu, out_dtype=t))
+            assert (np.abs(got - silu * b) <= most * (1 + step) + step * np.abs(silu * b) + 1e-30).all()
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 40, 130])
+def test_strides_and_alignment(llk, gpu, M):
+    """X at any row stride and element alignment, Y as a slice: what lies beside
+    it stays; codes, scales and zeros as slices."""
+    K, N, group = 328, 72, 64
+    x, codes, scales, z = case(gpu, M, K, N, group, True, gpu.bfloat16, M, True)
+    want = gpu.from_numpy(f64(x) @ dense(codes, scales, z, group)).float().cuda()
+
+    def wider(t, left, right):
+        big = gpu.full((t.shape[0], t.shape[1] + left + right), 99, device="cuda").to(t.dtype)
+        big[:, left:left + t.shape[1]] = t
+        return big[:, left:left + t.shape[1]]
+
+    w = llk.Q4Weights.from_codes(wider(codes, 3, 2), wider(scales, 1, 4), wider(z, 5, 1), group=group)
+    for left, right in ((1, 0), (3, 4), (8, 8)):
+        big = gpu.full((M + 2, N + 7), 5.0, device="cuda")
+        llk.q4_matmul(wider(x, left, right), w, out=big[1:-1, 2:2 + N])
+        assert gpu.equal(big[1:-1, 2:2 + N], want)
+        big[1:-1, 2:2 + N] = 5.0
+        assert (big == 5.0).all()
+
+
+def test_empty(llk, gpu):
+    x, codes, scales, z = case(gpu, 4, 64, 32, 32, False, gpu.bfloat16, 1, True)
+    w = llk.Q4Weights.from_codes(codes, scales, z, group=32)
+    assert llk.q4_matmul(x[:0], w).shape == (0, 32)
+    none = llk.Q4Weights.from_codes(codes[:0], scales[:0], group=32)
+    for M in (4, 40):
+        some = gpu.zeros(M, 0, dtype=gpu.bfloat16, device="cuda")
+        assert (llk.q4_matmul(some, none) == 0).all()
+        assert (llk.q4_swiglu(some, none, none) == 0).all()
+        acc = gpu.ones(M, 32, device="cuda")
+        assert (llk.q4_matmul(some, none, out=acc, accumulate=True) == 1).all()
+    narrow = llk.Q4Weights.from_codes(codes[:, :0], scales[:, :0], group=32)
+    assert llk.q4_matmul(x, narrow).shape == (4, 0)
+
+
+@pytest.mark.parametrize("M", [1, 6, 16, 50, 140])
+def test_non_finite_rows_stay_in_their_row(llk, gpu, M):
+    K, N, group = 200, 40, 64
+    x, codes, scales, z = case(gpu, M, K, N, group, True, gpu.bfloat16, 3, True)
+    w = llk.Q4Weights.from_codes(codes, scales, z, group=group)
+    want = llk.q4_matmul(x, w)
+    for bad in (float("inf"), float("nan")):
+        y = x.clone()
+        y[M // 2, 77] = bad
+        got = llk.q4_matmul(y, w)
+        assert got[M // 2].isnan().all()
+        rest = [m for m in range(M) if m != M // 2]
+        assert gpu.equal(got[rest], want[rest])
+    # a scale that is not finite stays in its column
+    s = scales.clone()
+    s[1, 7] = float("nan")
+    got = llk.q4_matmul(x, llk.Q4Weights.from_codes(codes, s, z, group=group))
+    assert got[:, 7].isnan().all()
+    keep = [n for n in range(N) if n != 7]
+    assert gpu.equal(got[:, keep], want[:, keep])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantise(llk, gpu, group):
+    """Codes, scales and zeros against the rule in fp32, value for value."""
+    gen = gpu.Generator(device="cuda").manual_seed(group)
+    for K, N in ((1, 1), (130, 257), (300, 70)):
+        w = gpu.randn(K, N, generator=gen, device="cuda").bfloat16()
+        w[:, 0] = 0
+        w[K // 2, N // 2] = 40.0
+        if N > 5:
+            w[0, 3], w[0, 4], w[0, 5] = float("nan"), float("inf"), 3e38
+        for zeros in (False, True):
+            for t in (gpu.bfloat16, gpu.float16):
+                codes, scales, z = llk.q4_quantise(w, group=group, zeros=zeros, scale_dtype=t)
+                assert (z is None) == (not zeros)
+                x = w.float().cpu().numpy()
+                for g in range(-(-K // group)):
+                    part = x[g * group:(g + 1) * group]
+                    lo, hi = np.minimum(part.min(0), 0), np.maximum(part.max(0), 0)
+                    f = np.float32
+                    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+                        s = hi / f(15) - lo / f(15) if zeros else np.maximum(hi, -lo) / f(7)
+                        s[~np.isfinite(part).all(0)] = np.nan
+                        s = gpu.from_numpy(s).to(t).float().numpy()
+                        some = (s > 0) & np.isfinite(s)
+                        zero = np.full(N, 8, f) if not zeros else \
+                            np.where(some, np.minimum(np.rint(-lo / s), 15), 0).astype(f)
+                        c = np.where(some, np.clip(np.rint(part / s) + zero, 0, 15), zero)
+                    assert np.array_equal(scales[g].float().cpu().numpy(), s, equal_nan=True)
+                    assert np.array_equal(codes[g * group:(g + 1) * group].cpu().numpy(), c)
+                    if zeros:
+                        assert np.array_equal(z[g].cpu().numpy(), zero)
+
+
+def test_quantised_weights(llk, gpu):
+    """Weights through quantise() and back: each within half a step."""
+    K, N, group = 256, 96, 64
+    w = gpu.randn(K, N, device="cuda").bfloat16()
+    eye = gpu.eye(K, device="cuda").bfloat16()
+    for zeros in (False, True):
+        codes, scales, z = llk.q4_quantise(w, group=group, zeros=zeros)
+        got = f64(llk.q4_matmul(eye, llk.Q4Weights.quantise(w, group=group, zeros=zeros)))
+        assert np.array_equal(got, dense(codes, scales, z, group))
+        # half a step, the zero's rounding by half a step more at the ends (held to
+        # 0..15), and the scale's by 2^-8 of at most 15 steps
+        step = f64(scales)[np.arange(K) // group]
+        assert (np.abs(got - f64(w)) <= step * (0.5 + 0.5 * zeros + 15 * 2.0 ** -8)).all()
+
+
+def test_streams_and_graph(llk, gpu):
+    """A captured product replays with new X; another stream gives the same."""
+    for M in (1, 12, 70):
+        x, codes, scales, z = case(gpu, M, 1000, 144, 128, True, gpu.float16, 5, False)
+        w = llk.Q4Weights.from_codes(codes, scales, z, group=128)
+        want = llk.q4_matmul(x, w)
+        side = gpu.cuda.Stream()
+        side.wait_stream(gpu.cuda.current_stream())
+        with gpu.cuda.stream(side):
+            assert gpu.equal(llk.q4_matmul(x, w), want)
+        got = gpu.empty_like(want)
+        gpu.cuda.synchronize()
+        llk.q4_matmul(x, w, out=got, stream=side)
+        side.synchronize()
+        assert gpu.equal(got, want)
+        graph = gpu.cuda.CUDAGraph()
+        with gpu.cuda.graph(graph, stream=side):
+            out = llk.q4_matmul(x, w)
+            both = llk.q4_swiglu(x, w, w)
+        for seed in range(3):
+            x.copy_(gpu.randn(*x.shape, device="cuda"))
+            graph.replay()
+            assert gpu.equal(out, llk.q4_matmul(x, w)) and gpu.equal(both, llk.q4_swiglu(x, w, w))
