@@ -141,6 +141,13 @@ class Q4WeightsC(C.Structure):
                 ("N", C.c_int64), ("group", C.c_int64)]
 
 
+class RotaryParams(C.Structure):
+    """llk_rotary_params."""
+    _fields_ = [("rotary_dim", C.c_int64), ("base", C.c_double), ("scaling", C.c_int),
+                ("factor", C.c_double), ("trained", C.c_double), ("fast", C.c_double),
+                ("slow", C.c_double)]
+
+
 class LLKError(RuntimeError):
     """A negative llk_status, with the library's message."""
 
@@ -206,6 +213,10 @@ SIGNATURES = {
     "llk_kv4_read": (C.c_int, [KC, KB, T3, T3, CTX]),
     "llk_kv4_attention": (C.c_int, [T3, KC, KB, AP, T3, CTX]),
     "llk_kv4_attention_describe": (C.c_int, [T3, KC, KB, AP, C.POINTER(AttentionPlan)]),
+    "llk_rotary_frequencies": (C.c_int, [C.POINTER(RotaryParams), C.POINTER(C.c_double),
+                                         C.POINTER(C.c_double)]),
+    "llk_rotary_turns": (C.c_int, [C.POINTER(C.c_double), C.c_int64, C.POINTER(C.c_uint64)]),
+    "llk_rotary": (C.c_int, [T3, T3, P, P, C.c_int64, C.c_float, C.c_int, C.c_int, T3, T3, CTX]),
     "llk_q4_code_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
     "llk_q4_scale_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
     "llk_q4_quantise": (C.c_int, [T2, C.c_int64, T2, T2, C.c_int, T2, CTX]),

@@ -53,14 +53,17 @@ HIP_SOURCES = [
     CSRC / "kernels" / "kv4_prompt.hip",
     CSRC / "kernels" / "q4_pack.hip",
     CSRC / "kernels" / "q4_gemv.hip",
+    CSRC / "kernels" / "rotary.hip",
     CSRC / "llk_abi.cpp",  # host code that calls the HIP runtime
     CSRC / "decoder_ops.cpp",
     CSRC / "q4_ops.cpp",
+    CSRC / "rotary_ops.cpp",
     CSRC / "kernel_fn.cpp",
     CSRC / "code_object.cpp",
 ]
 # Host sources built by hipcc (they call the HIP runtime or hold device data).
-HIP_HOST_SOURCES = {"llk_abi.cpp", "decoder_ops.cpp", "q4_ops.cpp", "kernel_fn.cpp", "code_object.cpp"}
+HIP_HOST_SOURCES = {"llk_abi.cpp", "decoder_ops.cpp", "q4_ops.cpp", "rotary_ops.cpp",
+                    "kernel_fn.cpp", "code_object.cpp"}
 # One code object per operation (kernels/code_object.hip with LLK_CO_OP),
 # named as code_object.cpp looks them up.
 CODE_OBJECTS = {"llk_fused_swiglu_gfx950.hsaco": 1, "llk_matmul_gfx950.hsaco": 0}

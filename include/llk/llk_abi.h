@@ -311,7 +311,7 @@ int llk_block_norm(const llk_tensor2d* y, const llk_tensor2d* residual,
                    llk_tensor2d* residual_out, llk_tensor2d* out,
                    const llk_block_norm_params* params, llk_kernel_context* ctx);
 
-/* bf16 [dim0, dim1, dim2] with unit stride2; stride0 and stride1 in elements,
+/* [dim0, dim1, dim2] (bf16 where nothing else is said) with unit stride2; stride0 and stride1 in elements,
  * in either order (rows of a result must not overlap). */
 typedef struct llk_tensor3d {
   void* data;
@@ -408,6 +408,51 @@ typedef struct llk_attention_plan {
 int llk_kv4_attention_describe(const llk_tensor3d* q, const llk_kv4_cache* cache,
                                const llk_kv4_batch* batch, const llk_attention_params* params,
                                llk_attention_plan* out);
+
+/* ----------------------------------------------------------------------- */
+/* Rotary positions (no counterpart in the reference)                       */
+/* ----------------------------------------------------------------------- */
+
+typedef enum llk_rotary_scaling {
+  LLK_ROTARY_PLAIN = 0,  /* f_i = base ^ (-2 i / rotary_dim), radians a position */
+  LLK_ROTARY_LINEAR = 1, /* f_i / factor */
+  LLK_ROTARY_BASE = 2,   /* of the base base * factor ^ (rotary_dim / (rotary_dim - 2)) */
+  LLK_ROTARY_YARN = 3,   /* r f_i / factor + (1 - r) f_i, r rising from 0 to 1 over the
+                            pairs from that of `fast` turns over `trained` positions
+                            (rounded down) to that of `slow` (rounded up) */
+  LLK_ROTARY_BANDS = 4   /* the same with 1 - r = (turns - slow) / (fast - slow), held to 0..1 */
+} llk_rotary_scaling;
+
+typedef struct llk_rotary_params {
+  int64_t rotary_dim; /* even, 2 to 1024 */
+  double base;
+  int scaling;        /* llk_rotary_scaling */
+  double factor;
+  double trained;
+  double fast, slow;
+} llk_rotary_params;
+
+/* The rotary_dim / 2 frequencies, and what the result is multiplied by unless the
+ * caller knows better (yarn: 0.1 ln(factor) + 1; otherwise 1).  Host only. */
+int llk_rotary_frequencies(const llk_rotary_params* params, double* frequencies,
+                           double* attention_factor);
+
+/* Frequencies as turns a position, f / (2 pi) modulo 1 in units of 2^-64: the
+ * table that llk_rotary reads (on the device).  Host only; 1 to 512 pairs. */
+int llk_rotary_turns(const double* frequencies, int64_t pairs, uint64_t* turns);
+
+#define LLK_ROTARY_INTERLEAVED 1 /* pairs (2 i, 2 i + 1); otherwise (i, i + pairs) */
+#define LLK_ROTARY_INVERSE 2     /* angles negated: the gradient of the call without it */
+
+/* q and k [tokens, heads, head_dim] of dtype LLK_BF16 or LLK_FP32, of every head
+ * the pairs among the first 2 * pairs values turned by positions[token] * f_i:
+ * (a cos - b sin, b cos + a sin) * factor; the others are copied.  positions
+ * (any) and turns are device memory.  k and k_out may be NULL.  q_out may be q and
+ * k_out k; otherwise results overlap nothing.  Angles are exact to 2^-24 of a turn
+ * at any position; arithmetic in fp32. */
+int llk_rotary(const llk_tensor3d* q, const llk_tensor3d* k, const int32_t* positions,
+               const uint64_t* turns, int64_t pairs, float factor, int dtype, int flags,
+               llk_tensor3d* q_out, llk_tensor3d* k_out, llk_kernel_context* ctx);
 
 /* ----------------------------------------------------------------------- */
 /* Weights in 4 bits (no counterpart in the reference)                      */
