@@ -141,6 +141,17 @@ class Q4WeightsC(C.Structure):
                 ("N", C.c_int64), ("group", C.c_int64)]
 
 
+class Kv4Marks(C.Structure):
+    """llk_kv4_marks."""
+    _fields_ = [("weights", C.c_void_p), ("positions", C.c_void_p), ("weights_stride", C.c_int64),
+                ("positions_stride", C.c_int64)]
+
+
+class EvictParams(C.Structure):
+    """llk_kv4_evict_params."""
+    _fields_ = [("keep", C.c_int64), ("recent", C.c_int64), ("first", C.c_int64)]
+
+
 class RotaryParams(C.Structure):
     """llk_rotary_params."""
     _fields_ = [("rotary_dim", C.c_int64), ("base", C.c_double), ("scaling", C.c_int),
@@ -165,6 +176,7 @@ KC = C.POINTER(Kv4Cache)
 KB = C.POINTER(Kv4Batch)
 AP = C.POINTER(AttentionParams)
 Q4 = C.POINTER(Q4WeightsC)
+KM = C.POINTER(Kv4Marks)
 KKP = C.POINTER(KernelKeyC)
 WKP = C.POINTER(WeightKeyC)
 # llk_kernel_fn: the shape of llk_swiglu_bf16
@@ -213,6 +225,12 @@ SIGNATURES = {
     "llk_kv4_read": (C.c_int, [KC, KB, T3, T3, CTX]),
     "llk_kv4_attention": (C.c_int, [T3, KC, KB, AP, T3, CTX]),
     "llk_kv4_attention_describe": (C.c_int, [T3, KC, KB, AP, C.POINTER(AttentionPlan)]),
+    "llk_kv4_write_marked": (C.c_int, [T3, T3, KC, KB, KM, P, CTX]),
+    "llk_kv4_attention_weigh": (C.c_int, [T3, KC, KB, AP, KM, C.c_float, T3, CTX]),
+    "llk_kv4_attention_weigh_describe": (C.c_int, [T3, KC, KB, AP, C.POINTER(AttentionPlan)]),
+    "llk_kv4_evict_plan": (C.c_int, [KM, C.c_int64, C.c_int64, C.c_int64, KB,
+                                     C.POINTER(EvictParams), P, P, CTX]),
+    "llk_kv4_evict": (C.c_int, [KC, KB, P, C.c_int64, KM, P, CTX]),
     "llk_rotary_frequencies": (C.c_int, [C.POINTER(RotaryParams), C.POINTER(C.c_double),
                                          C.POINTER(C.c_double)]),
     "llk_rotary_turns": (C.c_int, [C.POINTER(C.c_double), C.c_int64, C.POINTER(C.c_uint64)]),

@@ -167,6 +167,25 @@ int check_move(const llk_tensor3d* k, const llk_tensor3d* v, const llk_kv4_cache
   return *empty ? LLK_OK : llk::current_gfx950(&dev);
 }
 
+// Marks of a cache's slots.  need: 1 the weights, 2 the positions.
+int check_marks(const llk_kv4_marks* m, int64_t pages, int64_t heads, int64_t page_size, int need,
+                Kv4Marks* out) {
+  if (!m) return fail(LLK_ERR_INVALID_ARGUMENT, "marks is NULL");
+  if (((need & 1) && !m->weights) || ((need & 2) && !m->positions))
+    return fail(LLK_ERR_INVALID_ARGUMENT, "marks.%s is NULL",
+                (need & 1) && !m->weights ? "weights" : "positions");
+  if (reinterpret_cast<uintptr_t>(m->weights) % 4 || reinterpret_cast<uintptr_t>(m->positions) % 4)
+    return fail(LLK_ERR_LAYOUT, "marks are not aligned to their elements");
+  const int64_t least = heads * page_size;
+  if (pages > 1 && ((m->weights && m->weights_stride < least) ||
+                    (m->positions && m->positions_stride < least)))
+    return fail(LLK_ERR_LAYOUT, "a page stride of the marks (%lld, %lld) < %lld heads of %lld slots",
+                (long long)m->weights_stride, (long long)m->positions_stride, (long long)heads,
+                (long long)page_size);
+  *out = Kv4Marks{m->weights, m->positions, m->weights_stride, m->positions_stride};
+  return LLK_OK;
+}
+
 struct AttentionPlan {
   int rows;  // row tile
   int64_t tiles;
@@ -263,6 +282,53 @@ int check_attention(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk
   a->splits = plan->splits;
   a->chunk = plan->chunk;
   return LLK_OK;
+}
+
+// Where the rows' statistics lie in the workspace of an attention that adds its
+// weights up: after the splits' parts.
+size_t stats_at(const AttentionPlan& p) { return (p.bytes + 255) / 256 * 256; }
+size_t stats_bytes(const llk_tensor3d* q) { return (size_t)(q->dim0 * q->dim1) * 2 * sizeof(float); }
+
+// The sequences' heads are workgroups of up to 1024 threads along one dimension.
+int check_heads(const Kv4Batch& b, int64_t heads) {
+  constexpr int64_t kMost = ((int64_t)1 << 22) - 1;
+  return b.sequences * heads <= kMost
+             ? LLK_OK
+             : fail(LLK_ERR_SHAPE, "%d sequences of %lld heads are too many for one call (%lld)",
+                    b.sequences, (long long)heads, (long long)kMost);
+}
+
+int attend(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk_kv4_batch* batch,
+           const llk_attention_params* params, const llk_kv4_marks* marks, float decay,
+           llk_tensor3d* out, llk_kernel_context* ctx) {
+  Kv4AttentionArgs a{};
+  AttentionPlan p{};
+  Kv4Marks m{};
+  bool empty = false;
+  int rc = check_attention(q, cache, batch, params, &a, &p, &empty);
+  if (rc || (rc = check_rows3(out, "out", batch->tokens, q->dim1, cache->head_dim, true))) return rc;
+  if (marks) {
+    if ((rc = check_marks(marks, cache->pages, cache->heads, cache->page_size, 1, &m)) ||
+        (rc = check_heads(a.batch, cache->heads)))
+      return rc;
+    if (!(decay >= 0.0f) || !std::isfinite(decay))
+      return fail(LLK_ERR_INVALID_ARGUMENT, "decay %g is negative or not finite", decay);
+  }
+  if (empty) return LLK_OK;
+  a.out = bf16_of(out);
+  a.out_token = out->stride0;
+  a.out_head = out->stride1;
+  int dev;
+  if ((rc = llk::current_gfx950(&dev))) return rc;
+  llk::CallWorkspace ws;
+  if ((rc = ws.begin(dev, marks ? stats_at(p) + stats_bytes(q) : p.bytes, ctx))) return rc;
+  a.part = static_cast<float*>(ws.ptr());
+  if (marks) a.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(ws.ptr()) + stats_at(p));
+  hipError_t e = llk_launch_kv4_attention(a, (int)cache->head_dim, p.rows, stream_of(ctx));
+  if (marks && e == hipSuccess)
+    e = llk_launch_kv4_weigh(a, m, decay, (int)cache->head_dim, batch->max_len, stream_of(ctx));
+  ws.end();
+  return e == hipSuccess ? LLK_OK : fail_hip(e, "cache attention kernel");
 }
 
 }  // namespace
@@ -381,24 +447,115 @@ int llk_kv4_attention_describe(const llk_tensor3d* q, const llk_kv4_cache* cache
 int llk_kv4_attention(const llk_tensor3d* q, const llk_kv4_cache* cache,
                       const llk_kv4_batch* batch, const llk_attention_params* params,
                       llk_tensor3d* out, llk_kernel_context* ctx) {
-  Kv4AttentionArgs a{};
-  AttentionPlan p{};
+  return attend(q, cache, batch, params, nullptr, 0.0f, out, ctx);
+}
+
+int llk_kv4_write_marked(const llk_tensor3d* k, const llk_tensor3d* v, const llk_kv4_cache* cache,
+                         const llk_kv4_batch* batch, const llk_kv4_marks* marks, const int32_t* at,
+                         llk_kernel_context* ctx) {
+  Kv4Cache c;
+  Kv4Batch b;
+  Kv4Rows r;
+  Kv4Marks m;
   bool empty = false;
-  int rc = check_attention(q, cache, batch, params, &a, &p, &empty);
-  if (rc || (rc = check_rows3(out, "out", batch->tokens, q->dim1, cache->head_dim, true))) return rc;
+  int rc = check_move(k, v, cache, batch, false, &c, &b, &r, &empty);
+  if (rc || (rc = check_marks(marks, cache->pages, cache->heads, cache->page_size, 0, &m))) return rc;
   if (empty) return LLK_OK;
-  a.out = bf16_of(out);
-  a.out_token = out->stride0;
-  a.out_head = out->stride1;
+  const hipError_t e =
+      llk_launch_kv4_write(c, b, r, (int)cache->head_dim, stream_of(ctx), &m, at);
+  return e == hipSuccess ? LLK_OK : fail_hip(e, "cache write kernel");
+}
+
+int llk_kv4_attention_weigh(const llk_tensor3d* q, const llk_kv4_cache* cache,
+                            const llk_kv4_batch* batch, const llk_attention_params* params,
+                            const llk_kv4_marks* marks, float decay, llk_tensor3d* out,
+                            llk_kernel_context* ctx) {
+  if (!marks) return fail(LLK_ERR_INVALID_ARGUMENT, "marks is NULL");
+  return attend(q, cache, batch, params, marks, decay, out, ctx);
+}
+
+int llk_kv4_attention_weigh_describe(const llk_tensor3d* q, const llk_kv4_cache* cache,
+                                     const llk_kv4_batch* batch, const llk_attention_params* params,
+                                     llk_attention_plan* out) {
+  const int rc = llk_kv4_attention_describe(q, cache, batch, params, out);
+  if (rc || out->launches == 0) return rc;
+  AttentionPlan p{};
+  p.bytes = out->workspace_bytes;
+  out->launches += 1;
+  out->workspace_bytes = stats_at(p) + stats_bytes(q);
+  return LLK_OK;
+}
+
+int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads, int64_t page_size,
+                       const llk_kv4_batch* batch, const llk_kv4_evict_params* params,
+                       int32_t* lens, int32_t* source, llk_kernel_context* ctx) {
+  Kv4EvictPlan p{};
+  int rc;
+  if ((rc = check_batch(batch, &p.batch))) return rc;
+  if (!page_size_ok(page_size))
+    return fail(LLK_ERR_SHAPE, "page_size %lld unsupported (a power of two, 16 to 4096)",
+                (long long)page_size);
+  if (pages < 1 || pages > 0x7fffffff || heads < 1 || heads > 65535)
+    return fail(LLK_ERR_SHAPE, "marks of %lld pages and %lld heads unsupported", (long long)pages,
+                (long long)heads);
+  if (!params) return fail(LLK_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (params->keep < 1 || params->keep > kKv4MaxLength)
+    return fail(LLK_ERR_SHAPE, "keep %lld unsupported (1 to %d)", (long long)params->keep,
+                kKv4MaxLength);
+  if (params->recent < 0 || params->first < 0 || params->recent + params->first > params->keep ||
+      params->recent > params->keep || params->first > params->keep)
+    return fail(LLK_ERR_INVALID_ARGUMENT, "recent %lld and first %lld are negative or beyond keep %lld",
+                (long long)params->recent, (long long)params->first, (long long)params->keep);
+  const bool guarded = params->recent > 0 || params->first > 0;
+  if ((rc = check_marks(marks, pages, heads, page_size, guarded ? 3 : 1, &p.marks)) ||
+      (rc = check_heads(p.batch, heads)))
+    return rc;
+  if (batch->sequences == 0) return LLK_OK;
+  if (!lens || !source)
+    return fail(LLK_ERR_INVALID_ARGUMENT, "%s is NULL", lens ? "source" : "lens");
+  // every head's workgroup reads the old lengths
+  if (lens == batch->lens)
+    return fail(LLK_ERR_INVALID_ARGUMENT, "the new lengths must not replace batch.lens");
   int dev;
   if ((rc = llk::current_gfx950(&dev))) return rc;
-  llk::CallWorkspace ws;
-  if ((rc = ws.begin(dev, p.bytes, ctx))) return rc;
-  a.part = static_cast<float*>(ws.ptr());
-  const hipError_t e =
-      llk_launch_kv4_attention(a, (int)cache->head_dim, p.rows, stream_of(ctx));
-  ws.end();
-  return e == hipSuccess ? LLK_OK : fail_hip(e, "cache attention kernel");
+  if (!guarded) p.marks.positions = nullptr;
+  p.pages = (int)pages;
+  p.heads = (int)heads;
+  p.page_shift = __builtin_ctzll((unsigned long long)page_size);
+  p.keep = (int)params->keep;
+  p.recent = (int)params->recent;
+  p.first = (int)params->first;
+  p.lens = lens;
+  p.source = source;
+  const hipError_t e = llk_launch_kv4_evict_plan(p, batch->max_len, stream_of(ctx));
+  return e == hipSuccess ? LLK_OK : fail_hip(e, "eviction plan kernel");
+}
+
+int llk_kv4_evict(const llk_kv4_cache* cache, const llk_kv4_batch* batch, const int32_t* source,
+                  int64_t keep, const llk_kv4_marks* marks, int32_t* lens, llk_kernel_context* ctx) {
+  Kv4Cache c;
+  Kv4Batch b;
+  Kv4Marks m{};
+  int rc;
+  if ((rc = check_cache(cache, &c))) return rc;
+  if (!batch) return fail(LLK_ERR_INVALID_ARGUMENT, "batch is NULL");
+  llk_kv4_batch used = *batch;  // its table and sequences
+  used.lens = used.table;
+  used.starts = nullptr;
+  used.tokens = used.sequences;
+  if (used.table_pages == 0) used.sequences = used.tokens = 0;  // no slots
+  if ((rc = check_batch(&used, &b))) return rc;
+  if (keep < 1 || keep > kKv4MaxLength)
+    return fail(LLK_ERR_SHAPE, "keep %lld unsupported (1 to %d)", (long long)keep, kKv4MaxLength);
+  if (marks && (rc = check_marks(marks, cache->pages, cache->heads, cache->page_size, 0, &m))) return rc;
+  if ((rc = check_heads(b, cache->heads))) return rc;
+  if (b.sequences == 0) return LLK_OK;
+  if (!source) return fail(LLK_ERR_INVALID_ARGUMENT, "source is NULL");
+  int dev;
+  if ((rc = llk::current_gfx950(&dev))) return rc;
+  const hipError_t e = llk_launch_kv4_evict(c, b, m, source, (int)keep, lens, (int)cache->head_dim,
+                                            stream_of(ctx));
+  return e == hipSuccess ? LLK_OK : fail_hip(e, "eviction kernel");
 }
 
 }  // extern "C"

@@ -41,6 +41,14 @@ struct Kv4Batch {
   int sequences, tokens;
 };
 
+// What is kept of every slot beside the cache, [pages][heads][page_size] each (either
+// may be null): the attention weight it got, and its token's position.
+struct Kv4Marks {
+  float* weights;
+  int32_t* positions;
+  int64_t weights_page, positions_page;  // page strides in elements
+};
+
 struct Kv4AttentionArgs {
   Kv4Cache cache;
   Kv4Batch batch;
@@ -54,6 +62,7 @@ struct Kv4AttentionArgs {
   int tiles;          // row tiles (of all sequences)
   int splits, chunk;  // splits of a sequence's key steps, steps to a split
   float scale;        // of q.k, times log2(e)
+  float* stats;       // null, or [tokens][q heads][2]: a row's reference score and sum
 };
 
 // A dimension of a launch takes fewer than 2^32 threads (with more it runs some of
@@ -67,8 +76,11 @@ struct Kv4Rows {
   uint16_t *k, *v;
   int64_t k_token, k_head, v_token, v_head;
 };
+// marks: of the tokens that are written, weight 0 and position at[token] (null: the
+// slot's number).
 hipError_t llk_launch_kv4_write(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& rows, int D,
-                                hipStream_t s);
+                                hipStream_t s, const Kv4Marks* marks = nullptr,
+                                const int32_t* at = nullptr);
 hipError_t llk_launch_kv4_read(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& rows, int D,
                                hipStream_t s);
 
@@ -79,6 +91,24 @@ constexpr int kKv4PromptRows = 128;
 hipError_t llk_launch_kv4_prompt(const Kv4AttentionArgs& a, int D, hipStream_t s);
 hipError_t llk_launch_kv4_attention(const Kv4AttentionArgs& a, int D, int rows, hipStream_t s);
 size_t llk_kv4_attention_part_bytes(int64_t tiles, int heads, int splits, int rows, int D);
+
+// After an attention that left its rows' statistics: adds every key's weights up.
+hipError_t llk_launch_kv4_weigh(const Kv4AttentionArgs& a, const Kv4Marks& marks, float decay, int D,
+                                int64_t max_len, hipStream_t s);
+
+// Which slots of a sequence's heads stay, and where they come from.
+struct Kv4EvictPlan {
+  Kv4Marks marks;
+  Kv4Batch batch;
+  int pages, heads, page_shift;  // of the marks
+  int keep, recent, first;
+  int32_t* lens;    // [sequences]
+  int32_t* source;  // [sequences][heads][keep]
+};
+hipError_t llk_launch_kv4_evict_plan(const Kv4EvictPlan& p, int64_t max_len, hipStream_t s);
+hipError_t llk_launch_kv4_evict(const Kv4Cache& c, const Kv4Batch& b, const Kv4Marks& marks,
+                                const int32_t* source, int keep, int32_t* lens, int D,
+                                hipStream_t s);
 // Longest sequence (and window); positions and their sums fit 32 bits.
 constexpr int kKv4MaxLength = 1 << 30;
 // Keys that one step of a tile of `rows` rows covers.
@@ -111,22 +141,30 @@ __device__ __forceinline__ int kv4_sequence(const Kv4Batch& b, int t) {
   return lo;
 }
 
-// Where new token t of the call lies: its 16-token tile (of head 0) and its
-// number in it; false if it has no place (outside every sequence, before
-// position 0, past the table, on a page that does not exist).
-__device__ __forceinline__ bool kv4_place(const Kv4Cache& c, const Kv4Batch& b, int t,
-                                          int tile_bytes, uint8_t** tile, int* tok) {
+// Where new token t of the call lies: its position, page and slot in the page;
+// false if it has no place (outside every sequence, before position 0, past the
+// table, on a page that does not exist).
+__device__ __forceinline__ bool kv4_slot(const Kv4Cache& c, const Kv4Batch& b, int t, int* pos,
+                                         int* page, int* slot) {
   const int s = kv4_sequence(b, t);
   if (s >= b.sequences) return false;
   const int first = b.starts ? b.starts[s] : s, next = b.starts ? b.starts[s + 1] : s + 1;
   if (t < first || t >= next) return false;
-  const int64_t pos = (int64_t)b.lens[s] - (next - t);
-  if (pos < 0 || pos >= kKv4MaxLength || pos >= (int64_t)b.table_pages << c.page_shift) return false;
-  const int id = kv4_page(c, b, s, (int)pos);
-  if (id < 0) return false;
-  const int off = (int)pos & ((1 << c.page_shift) - 1);
-  *tile = c.data + id * c.page_stride + (int64_t)(off >> 4) * tile_bytes;
-  *tok = off & 15;
+  const int64_t p = (int64_t)b.lens[s] - (next - t);
+  if (p < 0 || p >= kKv4MaxLength || p >= (int64_t)b.table_pages << c.page_shift) return false;
+  *pos = (int)p;
+  *page = kv4_page(c, b, s, (int)p);
+  *slot = (int)p & ((1 << c.page_shift) - 1);
+  return *page >= 0;
+}
+
+// The same as its 16-token tile (of head 0) and its number in it.
+__device__ __forceinline__ bool kv4_place(const Kv4Cache& c, const Kv4Batch& b, int t,
+                                          int tile_bytes, uint8_t** tile, int* tok) {
+  int pos, page, slot;
+  if (!kv4_slot(c, b, t, &pos, &page, &slot)) return false;
+  *tile = c.data + page * c.page_stride + (int64_t)(slot >> 4) * tile_bytes;
+  *tok = slot & 15;
   return true;
 }
 

@@ -219,6 +219,16 @@ __device__ __forceinline__ float result(float o, float l, float inv) {
   return l == 0.0f ? 0.0f : o * inv;
 }
 
+// A row's statistics, for the call that adds its weights up: weight j is
+// exp2((score j - m) a.scale) / l.
+__device__ __forceinline__ void leave_stats(const Kv4AttentionArgs& a, const RowTile& rt, int head,
+                                            int row, float m, float l) {
+  if (!a.stats) return;
+  const int64_t at = (int64_t)(rt.token0 + row / a.group) * (a.cache.heads * a.group) +
+                     head * a.group + row % a.group;
+  reinterpret_cast<float2*>(a.stats)[at] = make_float2(m, l);
+}
+
 // Parts of a row's softmax (maximum m of the unscaled scores, sum l, 4 of the
 // unnormalised outputs) joined into one; m is the largest of theirs.
 struct Joined {
@@ -236,6 +246,7 @@ struct Joined {
                                         int r, int d) const {
     const int row = rt.row0 + r;
     const float inv = 1.0f / l;
+    if (d == 0) leave_stats(a, rt, head, row, m, l);
     uint16_t* dst = a.out + (int64_t)(rt.token0 + row / a.group) * a.out_token +
                     (int64_t)(head * a.group + row % a.group) * a.out_head + d;
     store8_any(dst, make_uint2(f32x2_to_bf16x2_rne(result(o[0], l, inv), result(o[1], l, inv)),

@@ -79,13 +79,26 @@ __device__ __forceinline__ uint32_t encode2(uint32_t codes, uint32_t two, float 
                                                    BYTE);
 }
 
-template <int D>
-__global__ void __launch_bounds__(kWaves * 64) kv4_write_kernel(Kv4Cache c, Kv4Batch b, Kv4Rows r) {
+// MARKS: the tokens' marks too.
+template <int D, bool MARKS>
+__global__ void __launch_bounds__(kWaves * 64)
+    kv4_write_kernel(Kv4Cache c, Kv4Batch b, Kv4Rows r, Kv4Marks marks, const int32_t* at) {
   const int lane = threadIdx.x & 63, quarter = lane & 3, t = blockIdx.x * 16 + (lane >> 2);
   uint8_t* tile = nullptr;
   int tok = 0;
   if (t >= b.tokens || !kv4_place(c, b, t, 17 * D, &tile, &tok)) return;
   const int blocks = c.heads * (D / 16);
+  if constexpr (MARKS) {
+    // a thread to a head of the token
+    int own, page = 0, slot = 0;
+    kv4_slot(c, b, t, &own, &page, &slot);
+    const int pos = at ? at[t] : own, size = 1 << c.page_shift;
+    for (int h = (blockIdx.y * kWaves + (threadIdx.x >> 6)) * 4 + quarter; h < c.heads;
+         h += gridDim.y * kWaves * 4) {
+      if (marks.weights) marks.weights[page * marks.weights_page + (int64_t)h * size + slot] = 0.0f;
+      if (marks.positions) marks.positions[page * marks.positions_page + (int64_t)h * size + slot] = pos;
+    }
+  }
   for (Walk w; w.c < blocks; w.c += kAhead * w.step) {
     u32x4 x[kAhead];
 #pragma unroll
@@ -164,21 +177,24 @@ __global__ void __launch_bounds__(kWaves * 64) kv4_read_kernel(Kv4Cache c, Kv4Ba
 // all, at least one block to a wave.
 template <class K>
 hipError_t launch_rows(K kernel, const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, int D,
-                       hipStream_t s) {
+                       hipStream_t s, const Kv4Marks* marks = nullptr, const int32_t* at = nullptr) {
   const unsigned groups = (unsigned)((b.tokens + 15) / 16);
   const unsigned most = (unsigned)(c.heads * (D / 16) + kWaves - 1) / kWaves;
   const unsigned y = std::min(std::max((2048 + groups - 1) / groups, 1u), std::min(most, 65535u));
   Kv4Cache ca = c;
   Kv4Batch ba = b;
   Kv4Rows ra = r;
-  void* params[] = {&ca, &ba, &ra};
+  Kv4Marks ma = marks ? *marks : Kv4Marks{};
+  void* params[] = {&ca, &ba, &ra, &ma, &at};  // (the read takes the first three)
   return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(groups, y), dim3(kWaves * 64),
                          params, 0, s);
 }
 
 template <int D>
-hipError_t write(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, hipStream_t s) {
-  return launch_rows(&kv4_write_kernel<D>, c, b, r, D, s);
+hipError_t write(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, const Kv4Marks* marks,
+                 const int32_t* at, hipStream_t s) {
+  return launch_rows(marks ? &kv4_write_kernel<D, true> : &kv4_write_kernel<D, false>, c, b, r, D, s,
+                     marks, at);
 }
 // From 64 MiB of keys and values on they are written past the L2.  8 heads of 128,
 // through the L2 and past it, us, into memory other than the last call's: 50 MB 14.2
@@ -196,9 +212,11 @@ hipError_t read(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, hipStrea
 }  // namespace llk_gfx950
 
 hipError_t llk_launch_kv4_write(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, int D,
-                                hipStream_t s) {
+                                hipStream_t s, const Kv4Marks* marks, const int32_t* at) {
   using namespace llk_gfx950;
-  return D == 64 ? write<64>(c, b, r, s) : D == 128 ? write<128>(c, b, r, s) : write<256>(c, b, r, s);
+  return D == 64    ? write<64>(c, b, r, marks, at, s)
+         : D == 128 ? write<128>(c, b, r, marks, at, s)
+                    : write<256>(c, b, r, marks, at, s);
 }
 
 hipError_t llk_launch_kv4_read(const Kv4Cache& c, const Kv4Batch& b, const Kv4Rows& r, int D,

@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(kTiles * 64)
             f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
   } else {
     const float inv = 1.0f / l;
+    if (half == 0) leave_stats(a, rt, head, rt.row0 + r, m, l);
     uint16_t* const dst = a.out + (int64_t)(rt.token0 + token) * a.out_token +
                           (int64_t)qhead * a.out_head + 4 * half;
 #pragma unroll

@@ -5,7 +5,9 @@
 - :func:`kv4_cache`, :func:`kv4_write`, :func:`kv4_read`: a paged cache of keys
   and values in 4 bits, quantised as it is written;
 - :func:`kv4_attention`: attention over that cache, for single tokens and for
-  prompts, with a sliding window and first positions that stay visible.
+  prompts, with a sliding window and first positions that stay visible;
+- :func:`kv4_marks`, :func:`kv4_evict_plan`, :func:`kv4_evict`: the attention
+  weight that each cached token got, and a cache bounded by it.
 
 The cache is a uint8 tensor [pages, heads, bytes] (the layout is in
 ``include/llk/llk_abi.h``), which may be a slice of a larger pool.  A call's
@@ -23,16 +25,17 @@ from .ops import _check_operand, _check_scratch, _torch
 
 _NO_GATE = _lib.Tensor2D(None, 0, 0, 0, 0)
 _get_device = _raw_stream = None  # torch's current device and its stream's handle
-_FLOATS = _BF16 = _INT32 = _UINT8 = None  # torch dtype -> llk_dtype (0 for the others)
+_FLOATS = _BF16 = _INT32 = _UINT8 = _FP32 = None  # torch dtype -> llk_dtype (0 for the others)
 
 
 def _begin() -> int:
     """The current device.  (A call of these operators is a few microseconds of
     GPU work in a decode step: the checks below take 0.2 us an operand.)"""
-    global _get_device, _raw_stream, _FLOATS, _BF16, _INT32, _UINT8
+    global _get_device, _raw_stream, _FLOATS, _BF16, _INT32, _UINT8, _FP32
     if _get_device is None:
         torch = _torch()
         _FLOATS = {torch.bfloat16: LLK_BF16, torch.float32: LLK_FP32}
+        _FP32 = {torch.float32: LLK_FP32}
         _BF16, _INT32, _UINT8 = {torch.bfloat16: LLK_BF16}, {torch.int32: 0}, {torch.uint8: 0}
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: int(torch.cuda.current_stream(d).cuda_stream))
@@ -190,14 +193,58 @@ def _rows3(t, name: str, dev: int) -> _lib.Tensor3D:
     return _lib.Tensor3D(t.data_ptr(), *t.shape, *t.stride())
 
 
-def kv4_write(k, v, cache, table, lens, *, starts=None, stream=None) -> None:
+def kv4_marks(pages: int, heads: int, page_size: int, device="cuda"):
+    """(weights fp32, positions int32) of a cache's slots, zeroed [pages, heads,
+    page_size]: the attention weight each slot's token got, and its position."""
+    torch = _torch()
+    shape = (pages, heads, page_size)
+    return (torch.zeros(shape, dtype=torch.float32, device=device),
+            torch.zeros(shape, dtype=torch.int32, device=device))
+
+
+def _marks(weights, positions, shape, dev: int) -> _lib.Kv4Marks:
+    """shape: (pages, heads, page_size) of the cache, or None: of the marks."""
+    c = _lib.Kv4Marks(None, None, 0, 0)
+    for name, t, kinds in (("weights", weights, _FP32), ("positions", positions, _INT32)):
+        if t is None:
+            continue
+        _kind(t, name, dev, kinds)
+        if t.dim() != 3 or tuple(t.shape) != (shape or tuple(t.shape)):
+            raise ValueError(f"{name} must be [pages, heads, page_size]" +
+                             (f" = {shape}" if shape else ""))
+        shape = tuple(t.shape)
+        step, head, one = t.stride()
+        if (shape[2] > 1 and one != 1) or (shape[1] > 1 and head != shape[2]):
+            raise ValueError(f"the heads of a page of {name} must be contiguous")
+        setattr(c, name, t.data_ptr())
+        setattr(c, name + "_stride", step)
+    return c
+
+
+def kv4_write(k, v, cache, table, lens, *, starts=None, weights=None, positions=None, at=None,
+              stream=None) -> None:
     """Quantises the new tokens' keys and values, bf16 [tokens, heads,
-    head_dim], into the cache; tokens without a place in it are skipped."""
+    head_dim], into the cache; tokens without a place in it are skipped.
+
+    With marks (:func:`kv4_marks`), those of the slots that are written are set:
+    `weights` to 0, `positions` to at[token], int32 (None: the slot's number)."""
     dev = _begin()
     kd = _rows3(k, "k", dev)
-    check(lib().llk_kv4_write(kd, _rows3(v, "v", dev), _cache(cache, kd.dim2, dev),
-                              _batch(table, lens, starts, kd.dim0, None, dev),
-                              _context(dev, stream)))
+    cd, batch = _cache(cache, kd.dim2, dev), _batch(table, lens, starts, kd.dim0, None, dev)
+    if weights is None and positions is None:
+        if at is not None:
+            raise ValueError("at without positions")
+        check(lib().llk_kv4_write(kd, _rows3(v, "v", dev), cd, batch, _context(dev, stream)))
+        return
+    marks = _marks(weights, positions, (cd.pages, cd.heads, cd.page_size), dev)
+    if at is not None:
+        _kind(at, "at", dev, _INT32)
+        if positions is None or at.dim() != 1 or at.shape[0] != kd.dim0 or (
+                kd.dim0 > 1 and at.stride(0) != 1):
+            raise ValueError("at must be a contiguous vector of the tokens' positions, for positions")
+        at = at.data_ptr()
+    check(lib().llk_kv4_write_marked(kd, _rows3(v, "v", dev), cd, batch, marks, at,
+                                     _context(dev, stream)))
 
 
 def kv4_read(cache, table, lens, *, head_dim: int, starts=None, tokens: int | None = None, k=None,
@@ -238,7 +285,7 @@ def _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev
 
 def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = None,
                   window: int = 0, sinks: int = 0, max_len: int | None = None, out=None,
-                  stream=None, scratch=None):
+                  weights=None, decay: float = 1.0, stream=None, scratch=None):
     """softmax(scale q k^T) v of the new tokens' queries, bf16 [tokens, q_heads,
     head_dim], over the cached keys and values.
 
@@ -248,7 +295,11 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
     sequence (padding of a captured step) are not written: what `out` held, or
     nothing defined.  max_len, if the caller knows it, is at least the longest
     of lens: the launch is planned by it (by the table's size otherwise), and
-    any value gives right results."""
+    any value gives right results.
+
+    weights (of :func:`kv4_marks`): in every slot of a sequence with new tokens,
+    decay times what was there (with 0 it is not read) plus the softmax weights
+    that the new tokens' query heads gave it."""
     dev = _begin()
     args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev)
     if out is None:
@@ -257,15 +308,79 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
         od = _lib.Tensor3D(out.data_ptr(), qd.dim0, qd.dim1, qd.dim2, qd.dim1 * qd.dim2, qd.dim2, 1)
     else:
         od = _rows3(out, "out", dev)
-    check(lib().llk_kv4_attention(*args, od, _context(dev, stream, scratch)))
+    if weights is None:
+        check(lib().llk_kv4_attention(*args, od, _context(dev, stream, scratch)))
+    else:
+        c = args[1]
+        marks = _marks(weights, None, (c.pages, c.heads, c.page_size), dev)
+        check(lib().llk_kv4_attention_weigh(*args, marks, decay, od, _context(dev, stream, scratch)))
     return out
 
 
+def kv4_evict_plan(weights, table, lens, keep: int, *, positions=None, recent: int = 0,
+                   first: int = 0, max_len: int | None = None, lens_out=None, stream=None):
+    """(new lens, source): which slots stay where a sequence has more than `keep`.
+
+    Of each head's slots stay the `recent` newest positions and those below
+    `first` (which need `positions`; recent + first <= keep), then those of the
+    largest weights, ties to the lowest slot.  source int32 [sequences, heads,
+    keep] names the slot each slot below keep takes its token from (itself, if it
+    does not change): slots below keep that stay are not moved, the others take
+    those from keep on that stay, both in order.  Nothing is moved, and lens stays
+    as it is (lens_out must be other memory)."""
+    dev = _begin()
+    marks = _marks(weights, positions, None, dev)
+    if weights is None:
+        raise ValueError("weights is required")
+    batch = _batch(table, lens, None, lens.shape[0], max_len, dev)
+    torch = _torch()
+    pages, heads, size = weights.shape
+    if lens_out is None:
+        lens_out = torch.empty(lens.shape, dtype=torch.int32, device=lens.device)
+    else:
+        _kind(lens_out, "lens_out", dev, _INT32)
+        if lens_out.shape != lens.shape or (lens.shape[0] > 1 and lens_out.stride(0) != 1):
+            raise ValueError("lens_out must be a contiguous vector like lens")
+    source = torch.empty((lens.shape[0], heads, max(keep, 0)), dtype=torch.int32, device=lens.device)
+    check(lib().llk_kv4_evict_plan(marks, pages, heads, size, batch,
+                                   _lib.EvictParams(keep, recent, first), lens_out.data_ptr(),
+                                   source.data_ptr(), _context(dev, stream)))
+    return lens_out, source
+
+
+def kv4_evict(cache, table, source, *, head_dim: int, weights=None, positions=None, lens=None,
+              stream=None) -> None:
+    """Moves the cache's tokens, and their marks if given, as `source` of
+    :func:`kv4_evict_plan` says; lens, if given, is cut to source's `keep` in
+    place.  The pages behind the new lengths are free."""
+    dev = _begin()
+    cd = _cache(cache, head_dim, dev)
+    marks = _marks(weights, positions, (cd.pages, cd.heads, cd.page_size), dev)
+    _kind(table, "table", dev, _INT32)
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be [sequences, pages] with unit inner stride")
+    n, pages = table.shape
+    _kind(source, "source", dev, _INT32)
+    if source.dim() != 3 or source.shape[:2] != (n, cd.heads) or not source.is_contiguous():
+        raise ValueError(f"source must be contiguous [{n}, {cd.heads}, keep]")
+    if lens is not None:
+        _kind(lens, "lens", dev, _INT32)
+        if lens.dim() != 1 or lens.shape[0] != n or (n > 1 and lens.stride(0) != 1):
+            raise ValueError("lens must be a contiguous vector of the sequences")
+        lens = lens.data_ptr()
+    batch = _lib.Kv4Batch(table.data_ptr(), table.stride(0), pages, None, None, n, n, 0)
+    check(lib().llk_kv4_evict(cd, batch, source.data_ptr(), source.shape[2], marks, lens,
+                              _context(dev, stream)))
+
+
 def describe_kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = None,
-                           window: int = 0, sinks: int = 0, max_len: int | None = None) -> dict:
-    """The launch kv4_attention chooses for these arguments."""
+                           window: int = 0, sinks: int = 0, max_len: int | None = None,
+                           weigh: bool = False) -> dict:
+    """The launch kv4_attention chooses for these arguments (weigh: with
+    `weights`)."""
     p = _lib.AttentionPlan()
-    check(lib().llk_kv4_attention_describe(
-        *_attention(q, cache, table, lens, starts, scale, window, sinks, max_len, _begin()), p))
+    describe = lib().llk_kv4_attention_weigh_describe if weigh else lib().llk_kv4_attention_describe
+    check(describe(*_attention(q, cache, table, lens, starts, scale, window, sinks, max_len, _begin()),
+                   p))
     return {"rows": p.rows, "splits": p.splits, "workgroups": p.workgroups,
             "launches": p.launches, "workspace_bytes": p.workspace_bytes}

@@ -409,6 +409,68 @@ int llk_kv4_attention_describe(const llk_tensor3d* q, const llk_kv4_cache* cache
                                const llk_kv4_batch* batch, const llk_attention_params* params,
                                llk_attention_plan* out);
 
+/* What is kept of every slot of a cache beside it, in caller-owned device memory:
+ * the attention weight that the slot's token got, and the position that it came
+ * from (a slot's number is no position any more once others were evicted).
+ * [pages][heads][page_size] each, pages at any stride; either may be NULL where a
+ * call does not need it. */
+typedef struct llk_kv4_marks {
+  float* weights;
+  int32_t* positions;
+  int64_t weights_stride;   /* elements from page to page */
+  int64_t positions_stride;
+} llk_kv4_marks;
+
+/* llk_kv4_write that also sets the marks of the slots it writes: weight 0, and
+ * position at[token] (device memory; NULL: the slot's number in its sequence). */
+int llk_kv4_write_marked(const llk_tensor3d* k, const llk_tensor3d* v, const llk_kv4_cache* cache,
+                         const llk_kv4_batch* batch, const llk_kv4_marks* marks, const int32_t* at,
+                         llk_kernel_context* ctx);
+
+/* llk_kv4_attention that also adds up what weight every slot got: for each
+ * sequence with new tokens, each of its first lens[s] slots and each head,
+ *   marks.weights = decay * marks.weights + sum of the softmax weights that the new
+ *   tokens' query heads of that head gave the slot (0 from those that do not see it);
+ * with decay 0 what was there is not read.  In fp32, and the same from run to run.
+ * Other slots are left as they are.  A row without a key it sees adds nothing, one
+ * that is NaN makes the slots that it sees NaN.  The result is that of
+ * llk_kv4_attention, bit for bit. */
+int llk_kv4_attention_weigh(const llk_tensor3d* q, const llk_kv4_cache* cache,
+                            const llk_kv4_batch* batch, const llk_attention_params* params,
+                            const llk_kv4_marks* marks, float decay, llk_tensor3d* out,
+                            llk_kernel_context* ctx);
+/* Its launch, as llk_kv4_attention_describe gives that of llk_kv4_attention. */
+int llk_kv4_attention_weigh_describe(const llk_tensor3d* q, const llk_kv4_cache* cache,
+                                     const llk_kv4_batch* batch, const llk_attention_params* params,
+                                     llk_attention_plan* out);
+
+typedef struct llk_kv4_evict_params {
+  int64_t keep;   /* slots that stay of each head; at least 1 */
+  int64_t recent; /* positions above the sequence's newest minus this stay */
+  int64_t first;  /* positions below this stay; recent + first <= keep */
+} llk_kv4_evict_params;
+
+/* Which slots stay of every sequence with more than `keep`, a head at a time: the
+ * protected positions, then those of the largest weights, ties to the lowest slot
+ * (a NaN is below -infinity, a slot without a page below that; positions are
+ * not read where nothing is protected).  Slots below keep that stay are not moved;
+ * the others below keep, in order, take those from keep on that stay, in order:
+ * source[s][head][i], int32 [sequences][heads][keep], is the slot that slot i takes
+ * its token from, i itself if it does not change.  lens: the new lengths, the
+ * smaller of batch.lens and keep (not batch.lens itself, which every head reads).  Of batch, table,
+ * lens and sequences are read.  Nothing is moved. */
+int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads, int64_t page_size,
+                       const llk_kv4_batch* batch, const llk_kv4_evict_params* params,
+                       int32_t* lens, int32_t* source, llk_kernel_context* ctx);
+
+/* Moves tokens to the slots below `keep` as `source` (of llk_kv4_evict_plan) says,
+ * keys and values and, unless NULL, marks.  Slots are moved only from keep on, and
+ * only where both pages exist.  lens, unless NULL: lengths on the device that are
+ * cut to keep.  The pages behind the new lengths are the caller's again.  Of batch,
+ * table and sequences are read. */
+int llk_kv4_evict(const llk_kv4_cache* cache, const llk_kv4_batch* batch, const int32_t* source,
+                  int64_t keep, const llk_kv4_marks* marks, int32_t* lens, llk_kernel_context* ctx);
+
 /* ----------------------------------------------------------------------- */
 /* Rotary positions (no counterpart in the reference)                       */
 /* ----------------------------------------------------------------------- */
