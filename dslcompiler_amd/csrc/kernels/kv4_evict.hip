@@ -3,13 +3,14 @@
 //
 // Plan: a workgroup to a sequence's head.  The slots' order is that of a 32-bit key:
 // the weight's bits, turned so that they order like numbers, under the largest key
-// for the protected ones.  The `keep`-th largest key is found digit by digit (8 bits,
-// counts in LDS), and of those equal to it the lowest slots stay.  Slots below `keep`
+// for the protected ones.  The `keep`-th largest key is found from its upper bits
+// down, and of those equal to it the lowest slots stay.  Slots below `keep`
 // that stay are not moved: the holes among them take, in order, those from `keep` on
 // that stay.  So few bytes move however long the cache is, and none is read after it
 // was written: sources lie from `keep` on, targets below.
 //
-// Move: a wave to 64 slots below `keep`; 16 codes' bytes and their scale to a lane.
+// Move: a lane to a slot below `keep`, with all of its token's blocks on their way at
+// once.
 #include <algorithm>
 
 #include "common.h"
@@ -17,8 +18,6 @@
 
 namespace llk_gfx950 {
 namespace {
-
-constexpr int kThreads = 1024, kPlanWaves = kThreads / 64;
 
 struct Slots {  // of a sequence's head
   const Kv4EvictPlan& p;
@@ -46,7 +45,8 @@ struct Slots {  // of a sequence's head
 };
 
 // Sum over the workgroup, and of the threads before this one.
-__device__ __forceinline__ int scan(int x, int* before, int* part) {
+template <int WAVES>
+__device__ __forceinline__ int scan_threads(int x, int* before, int* part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int mine = x;
 #pragma unroll
@@ -57,7 +57,8 @@ __device__ __forceinline__ int scan(int x, int* before, int* part) {
   if (lane == 63) part[wave] = mine;
   __syncthreads();
   int all = 0, base = 0;
-  for (int w = 0; w < kPlanWaves; ++w) {
+#pragma unroll 1
+  for (int w = 0; w < WAVES; ++w) {
     base += w < wave ? part[w] : 0;
     all += part[w];
   }
@@ -66,23 +67,19 @@ __device__ __forceinline__ int scan(int x, int* before, int* part) {
   return all;
 }
 
-__global__ void __launch_bounds__(kThreads) kv4_evict_plan_kernel(Kv4EvictPlan p) {
-  __shared__ int counts[256], part[kPlanWaves];
+// Any length: the keys are read from memory at every pass.
+template <int THREADS>
+__device__ __forceinline__ void plan_long(const Kv4EvictPlan& p, int s, int head, int n,
+                                          int32_t* source) {
+  __shared__ int counts[256], part[THREADS / 64];
   __shared__ int shared_last, shared_digit, shared_above;
-  const int s = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
-  const int64_t cap = min((int64_t)p.batch.table_pages << p.page_shift, (int64_t)kKv4MaxLength);
-  const int n = (int)max((int64_t)0, min((int64_t)p.batch.lens[s], cap));
-  int32_t* const source = p.source + ((int64_t)s * p.heads + head) * p.keep;
-  if (head == 0 && threadIdx.x == 0) p.lens[s] = min(p.batch.lens[s], p.keep);
-  for (int j = threadIdx.x + (n > p.keep ? p.keep : 0); j < p.keep; j += kThreads) source[j] = j;
-  if (n <= p.keep) return;
   Slots slots{p, p.batch.table + s * p.batch.table_stride, head, 0};
 
   if (p.marks.positions) {  // the newest position
     if (threadIdx.x == 0) shared_last = INT32_MIN;
     __syncthreads();
     int last = INT32_MIN;
-    for (int j = threadIdx.x; j < n; j += kThreads) {
+    for (int j = threadIdx.x; j < n; j += THREADS) {
       int64_t page;
       int off;
       if (slots.at(j, &page, &off))
@@ -97,9 +94,9 @@ __global__ void __launch_bounds__(kThreads) kv4_evict_plan_kernel(Kv4EvictPlan p
   uint32_t key = 0;
   int left = p.keep;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) counts[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 256; i += THREADS) counts[i] = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < n; j += kThreads) {
+    for (int j = threadIdx.x; j < n; j += THREADS) {
       const uint32_t k = slots.key(j);
       if (shift == 24 || (k ^ key) >> (shift + 8) == 0) atomicAdd(&counts[k >> shift & 255], 1);
     }
@@ -123,17 +120,17 @@ __global__ void __launch_bounds__(kThreads) kv4_evict_plan_kernel(Kv4EvictPlan p
     const uint32_t k = j < bound ? slots.key(j) : 0;
     int before;
     const int same = j < bound && k == key;
-    const int all = scan(same, &before, part);
+    const int all = scan_threads<THREADS / 64>(same, &before, part);
     const bool stay = j < bound && (k > key || (same && equal + before < left));
     equal += all;
     return stay;
   };
-  for (int j0 = 0; j0 < p.keep; j0 += kThreads) stays(j0 + threadIdx.x, p.keep);
+  for (int j0 = 0; j0 < p.keep; j0 += THREADS) stays(j0 + threadIdx.x, p.keep);
   const int below = equal;
-  for (int j0 = p.keep; j0 < n; j0 += kThreads) {
+  for (int j0 = p.keep; j0 < n; j0 += THREADS) {
     const bool stay = stays(j0 + threadIdx.x, n);
     int before;
-    const int all = scan(stay, &before, part);
+    const int all = scan_threads<THREADS / 64>(stay, &before, part);
     if (stay) source[extras + before] = j0 + threadIdx.x;
     extras += all;
   }
@@ -142,19 +139,237 @@ __global__ void __launch_bounds__(kThreads) kv4_evict_plan_kernel(Kv4EvictPlan p
   // source[i], which no slot after the round has any use for.
   int holes = extras;  // in this round and before it
   equal = below;
-  for (int j0 = (p.keep - 1) / kThreads * kThreads; j0 >= 0; j0 -= kThreads) {
+  for (int j0 = (p.keep - 1) / THREADS * THREADS; j0 >= 0; j0 -= THREADS) {
     const int j = j0 + threadIdx.x;
     const uint32_t k = j < p.keep ? slots.key(j) : 0;
     const int same = j < p.keep && k == key;
     int before, nth;
-    equal -= scan(same, &before, part);
+    equal -= scan_threads<THREADS / 64>(same, &before, part);
     const bool hole = j < p.keep && !(k > key || (same && equal + before < left));
-    holes -= scan(hole, &nth, part);
+    holes -= scan_threads<THREADS / 64>(hole, &nth, part);
     const int from = hole ? source[holes + nth] : j;
     __syncthreads();
     if (j < p.keep) source[j] = from;
     __syncthreads();
   }
+}
+
+// Sum over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ uint32_t row_sum(uint32_t x) {
+  x += __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true);  // row_ror:8
+  x += __builtin_amdgcn_mov_dpp(x, 0x124, 0xf, 0xf, true);
+  x += __builtin_amdgcn_mov_dpp(x, 0x122, 0xf, 0xf, true);
+  x += __builtin_amdgcn_mov_dpp(x, 0x121, 0xf, 0xf, true);
+  return x;
+}
+
+// Sums over the lanes up to this one, in DPP steps.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
+// Up to PER * THREADS slots: the keys stay in registers, slot THREADS i + t in thread
+// t's i-th.  The keep-th largest is found by its upper 11 bits, then the next 11 and
+// the last 10, each time by counting the keys that agree so far in LDS (a weight's
+// sign, exponent and two bits of its mantissa spread over enough counters that lanes
+// seldom meet).  GUARD: some positions are protected.
+template <int PER, int THREADS, bool GUARD>
+__device__ __forceinline__ void plan_short(const Kv4EvictPlan& p, int s, int head, int n,
+                                           int32_t* source) {
+  constexpr int kWaves = THREADS / 64, kParts = PER * kWaves;
+  static_assert(kWaves <= 16 && PER * THREADS <= 16384, "counts and slots of 16 bits");
+  constexpr int kBins = 2048, kOwn = kBins / THREADS;  // counters, and of a thread
+  __shared__ int bins[kBins];
+  __shared__ int totals[16];  // of the waves
+  __shared__ int found[3];
+  __shared__ uint32_t part[kParts];
+  __shared__ uint16_t extra[PER * THREADS / 2];
+  __shared__ int newest;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int32_t* const table = p.batch.table + s * p.batch.table_stride;
+  // (slots past n read slot n - 1's, absent ones page 0's marks: all loads are in
+  // flight at once)
+  const int inner = (1 << p.page_shift) - 1;
+  int page[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) page[i] = table[min(i * THREADS + t, n - 1) >> p.page_shift];
+  float w[PER];
+  int pos[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool here = page[i] >= 0 && page[i] < p.pages;
+    const int64_t id = here ? page[i] : 0;
+    const int off = (head << p.page_shift) + (min(i * THREADS + t, n - 1) & inner);
+    w[i] = p.marks.weights[id * p.marks.weights_page + off];
+    if constexpr (GUARD) pos[i] = p.marks.positions[id * p.marks.positions_page + off];
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) bins[i * THREADS + t] = 0;
+  if (t < 16) totals[t] = 0;
+  int last = INT32_MIN;
+  if constexpr (GUARD) {
+    if (t == 0) newest = INT32_MIN;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      last = max(last, page[i] >= 0 && page[i] < p.pages ? pos[i] : INT32_MIN);
+    atomicMax(&newest, last);
+    __syncthreads();
+    last = __builtin_amdgcn_readfirstlane(newest);
+  }
+  // positions from here on are protected
+  const int64_t cut = (int64_t)last - p.recent + 1;
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t u = __float_as_uint(w[i] + 0.0f);  // -0 as 0
+    key[i] = u >> 31 ? ~u : u | 0x80000000u;
+    if (w[i] != w[i]) key[i] = 1;
+    if constexpr (GUARD) {
+      if (pos[i] >= cut || pos[i] < p.first) key[i] = 0xffffffffu;
+    }
+    if (page[i] < 0 || page[i] >= p.pages || i * THREADS + t >= n) key[i] = 0;
+  }
+  __syncthreads();
+
+  // `least`: the bits seen so far of the keep-th largest key, and zeros.  `reach`
+  // keys are not below it; `left` of those that agree with it are to stay.  Slots
+  // past n have the key 0, as absent ones, and the last places.
+  uint32_t least = 0;
+  int reach = 0, left = p.keep;
+#pragma unroll
+  for (int shift = 21, width = 11; shift >= 0; width = shift == 10 ? 10 : 11, shift -= width) {
+    const uint32_t mask = (1u << width) - 1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (shift == 21 || (key[i] ^ least) >> (shift + width) == 0)
+        atomicAdd(&bins[mask - (key[i] >> shift & mask)], 1);
+    __syncthreads();
+    int mine[kOwn], all = 0;  // counters from the largest digit on
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      mine[i] = bins[t * kOwn + i];
+      bins[t * kOwn + i] = 0;
+      all += mine[i];
+    }
+    const int up_to = wave_scan(all);
+    if (lane == 63) totals[wave] = up_to;
+    __syncthreads();
+    int base = (lane & 15) < wave ? totals[lane & 15] : 0;
+    base = (int)row_sum((uint32_t)base);
+    int before = base + up_to - all;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (before < left && left <= before + mine[i]) {
+        found[0] = (int)mask - (t * kOwn + i);
+        found[1] = before;
+        found[2] = mine[i];
+      }
+      before += mine[i];
+    }
+    __syncthreads();
+    least |= (uint32_t)__builtin_amdgcn_readfirstlane(found[0]) << shift;
+    const int above = __builtin_amdgcn_readfirstlane(found[1]);
+    const int same = __builtin_amdgcn_readfirstlane(found[2]);
+    reach = p.keep - left + above + same;
+    left -= above;
+    if (reach == p.keep) break;  // all that agree stay
+  }
+
+  // part to the sums before each entry
+  auto scan = [&] {
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t base = 0;
+#pragma unroll
+      for (int i = 0; i < kParts; i += 64) {
+        const int v = i + lane < kParts ? (int)part[i + lane] : 0, up_to = wave_scan(v);
+        if (i + lane < kParts) part[i + lane] = base + up_to - v;
+        base += __builtin_amdgcn_readlane(up_to, 63);
+      }
+    }
+    __syncthreads();
+  };
+  auto before = [&](uint64_t mask) {  // lanes of it before this one
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                     __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+  };
+  uint32_t stays = 0;  // bit i: the thread's i-th slot
+#pragma unroll
+  for (int i = 0; i < PER; ++i) stays |= (uint32_t)(key[i] >= least) << i;
+  if (reach != p.keep) {
+    // All bits are seen, and more keys are equal to the keep-th largest than stay:
+    // the lowest slots of them, `left`.
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t same = (uint32_t)__popcll(__ballot(key[i] == least));
+      if (lane == 0) part[i * kWaves + wave] = same;
+    }
+    scan();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int nth = (int)(part[i * kWaves + wave] + before(__ballot(key[i] == least)));
+      if (key[i] == least && nth >= left) stays &= ~(1u << i);
+    }
+    __syncthreads();
+  }
+  // holes below keep in the lower half of a count, those from keep on that stay in
+  // the upper
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool low = i * THREADS + t < p.keep, stay = stays >> i & 1;
+    const uint32_t holes = (uint32_t)__popcll(__ballot(low && !stay));
+    const uint32_t more = (uint32_t)__popcll(__ballot(!low && stay));
+    if (lane == 0) part[i * kWaves + wave] = holes | more << 16;
+  }
+  scan();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool more = i * THREADS + t >= p.keep && (stays >> i & 1);
+    const uint32_t nth = (part[i * kWaves + wave] >> 16) + before(__ballot(more));
+    if (more) extra[nth] = (uint16_t)(i * THREADS + t);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = i * THREADS + t;
+    const bool hole = j < p.keep && !(stays >> i & 1);
+    const uint32_t nth = (part[i * kWaves + wave] & 0xffffu) + before(__ballot(hole));
+    if (j < p.keep) source[j] = hole ? extra[nth] : j;
+  }
+}
+
+template <int PER, int THREADS, bool GUARD>
+__global__ void __launch_bounds__(THREADS)
+    __attribute__((amdgpu_waves_per_eu(PER <= 8 ? 8 : 4))) kv4_evict_plan_kernel(Kv4EvictPlan p) {
+  const int s = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+  const int64_t cap = min((int64_t)p.batch.table_pages << p.page_shift, (int64_t)kKv4MaxLength);
+  const int n = (int)max((int64_t)0, min((int64_t)p.batch.lens[s], cap));
+  int32_t* const source = p.source + ((int64_t)s * p.heads + head) * p.keep;
+  if (head == 0 && threadIdx.x == 0) p.lens[s] = min(p.batch.lens[s], p.keep);
+  if (n <= p.keep) {
+    for (int j = threadIdx.x; j < p.keep; j += THREADS) source[j] = j;
+    return;
+  }
+  if (n <= PER * THREADS) plan_short<PER, THREADS, GUARD>(p, s, head, n, source);
+  else plan_long<THREADS>(p, s, head, n, source);
+}
+
+template <int PER, int THREADS>
+hipError_t plan(const Kv4EvictPlan& args, hipStream_t s) {
+  Kv4EvictPlan p = args;
+  void* params[] = {&p};
+  return hipLaunchKernel(
+      p.marks.positions ? reinterpret_cast<const void*>(&kv4_evict_plan_kernel<PER, THREADS, true>)
+                        : reinterpret_cast<const void*>(&kv4_evict_plan_kernel<PER, THREADS, false>),
+      dim3((unsigned)(p.batch.sequences * p.heads)), dim3(THREADS), params, 0, s);
 }
 
 constexpr int kMoveWaves = 4;
@@ -163,7 +378,6 @@ template <int D>
 __global__ void __launch_bounds__(kMoveWaves * 64)
     kv4_evict_kernel(Kv4Cache c, Kv4Batch b, Kv4Marks marks, const int32_t* source, int keep,
                      int32_t* lens) {
-  __shared__ int2 moves[kMoveWaves][64];
   constexpr int kBlocks = D / 16;  // of a token's key and value
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int s = blockIdx.x / c.heads, head = blockIdx.x % c.heads;
@@ -172,56 +386,46 @@ __global__ void __launch_bounds__(kMoveWaves * 64)
   const int32_t* const from = source + ((int64_t)s * c.heads + head) * keep;
   const int size = 1 << c.page_shift;
   if (lens && head == 0 && blockIdx.y == 0 && threadIdx.x == 0) lens[s] = min(lens[s], keep);
-  for (int j0 = (blockIdx.y * kMoveWaves + wave) * 64; j0 < keep; j0 += gridDim.y * kMoveWaves * 64) {
-    const int j = j0 + lane, src = j < keep ? from[j] : j;
+  for (int j = (blockIdx.y * kMoveWaves + wave) * 64 + lane; j < keep; j += gridDim.y * kMoveWaves * 64) {
+    const int src = from[j];
     // (a source below keep could be a target itself: never one of a plan's)
-    const bool moved = src != j && src >= keep && src < cap && j < cap;
-    const uint64_t mask = __ballot(moved);
-    if (moved) moves[wave][__popcll(mask & ((1ull << lane) - 1))] = make_int2(j, src);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int all = __popcll(mask) * kBlocks;
-    for (int i = lane; i < all; i += 64) {
-      const int2 m = moves[wave][i / kBlocks];
-      const int part = i % kBlocks / (kBlocks / 2), block = i % (kBlocks / 2);
-      const int to = table[m.x >> c.page_shift], of = table[m.y >> c.page_shift];
-      if (to < 0 || to >= c.pages || of < 0 || of >= c.pages) continue;
-      auto at = [&](int page, int slot) {
-        return c.data + page * c.page_stride + head * c.head_bytes +
-               (int64_t)((slot & (size - 1)) >> 4) * (17 * D);
-      };
-      uint8_t* const dst = at(to, m.x);
-      const uint8_t* const org = at(of, m.y);
-      const int code = part * 8 * D + block * 256, scale = 16 * D + part * (D / 2) + block * 16;
-      *reinterpret_cast<u32x4*>(dst + code + (m.x & 15) * 16) =
-          *reinterpret_cast<const u32x4*>(org + code + (m.y & 15) * 16);
-      dst[scale + (m.x & 15)] = org[scale + (m.y & 15)];
-      if (i % kBlocks == 0) {
-        const int64_t dm = (int64_t)head * size + (m.x & (size - 1));
-        const int64_t om = (int64_t)head * size + (m.y & (size - 1));
-        if (marks.weights)
-          marks.weights[to * marks.weights_page + dm] = marks.weights[of * marks.weights_page + om];
-        if (marks.positions)
-          marks.positions[to * marks.positions_page + dm] =
-              marks.positions[of * marks.positions_page + om];
-      }
+    if (src == j || src < keep || src >= cap || j >= cap) continue;
+    const int to = table[j >> c.page_shift], of = table[src >> c.page_shift];
+    if (to < 0 || to >= c.pages || of < 0 || of >= c.pages) continue;
+    const int x = j & (size - 1), y = src & (size - 1);
+    uint8_t* const dst = c.data + to * c.page_stride + head * c.head_bytes + (int64_t)(x >> 4) * (17 * D);
+    const uint8_t* const org =
+        c.data + of * c.page_stride + head * c.head_bytes + (int64_t)(y >> 4) * (17 * D);
+    const int64_t dm = (int64_t)head * size + x, om = (int64_t)head * size + y;
+    u32x4 codes[kBlocks];
+    uint8_t scales[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      codes[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(org + i * 256 + (y & 15) * 16));
+      scales[i] = org[16 * D + i * 16 + (y & 15)];
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    float w = 0.0f;
+    int pos = 0;
+    if (marks.weights) w = marks.weights[of * marks.weights_page + om];
+    if (marks.positions) pos = marks.positions[of * marks.positions_page + om];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      *reinterpret_cast<u32x4*>(dst + i * 256 + (x & 15) * 16) = codes[i];
+      dst[16 * D + i * 16 + (x & 15)] = scales[i];
+    }
+    if (marks.weights) marks.weights[to * marks.weights_page + dm] = w;
+    if (marks.positions) marks.positions[to * marks.positions_page + dm] = pos;
   }
 }
 
 }  // namespace
 }  // namespace llk_gfx950
 
-hipError_t llk_launch_kv4_evict_plan(const Kv4EvictPlan& plan, int64_t, hipStream_t s) {
-  Kv4EvictPlan p = plan;
-  void* params[] = {&p};
-  return hipLaunchKernel(reinterpret_cast<const void*>(&llk_gfx950::kv4_evict_plan_kernel),
-                         dim3((unsigned)(p.batch.sequences * p.heads)), dim3(llk_gfx950::kThreads),
-                         params, 0, s);
+hipError_t llk_launch_kv4_evict_plan(const Kv4EvictPlan& p, int64_t max_len, hipStream_t s) {
+  using namespace llk_gfx950;
+  int64_t len = (int64_t)p.batch.table_pages << p.page_shift;
+  if (max_len > 0) len = std::min(len, max_len);
+  return len <= 2048 ? plan<2, 1024>(p, s) : len <= 8192 ? plan<8, 1024>(p, s) : plan<16, 1024>(p, s);
 }
 
 hipError_t llk_launch_kv4_evict(const Kv4Cache& cache, const Kv4Batch& batch, const Kv4Marks& m,
