@@ -237,6 +237,7 @@ SIGNATURES = {
     "llk_rotary": (C.c_int, [T3, T3, P, P, C.c_int64, C.c_float, C.c_int, C.c_int, T3, T3, CTX]),
     "llk_q4_code_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
     "llk_q4_scale_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "llk_q4_scratch_size": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
     "llk_q4_quantise": (C.c_int, [T2, C.c_int64, T2, T2, C.c_int, T2, CTX]),
     "llk_q4_pack": (C.c_int, [T2, T2, C.c_int, T2, Q4, CTX]),
     "llk_q4_gemm": (C.c_int, [T2, Q4, T2, C.c_int, C.c_int, CTX]),

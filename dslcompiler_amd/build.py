@@ -53,6 +53,7 @@ HIP_SOURCES = [
     CSRC / "kernels" / "kv4_prompt.hip",
     CSRC / "kernels" / "q4_pack.hip",
     CSRC / "kernels" / "q4_gemv.hip",
+    CSRC / "kernels" / "q4_tile.hip",
     CSRC / "kernels" / "kv4_weigh.hip",
     CSRC / "kernels" / "kv4_evict.hip",
     CSRC / "kernels" / "rotary.hip",

@@ -38,6 +38,15 @@ struct Q4Side {
   const uint32_t* scales;
 };
 
+// The launch of a product.
+struct Q4Plan {
+  int rows;      // to a workgroup: 16 (the kernel for few rows), 32 or 64
+  int splits;    // of K, joined by a second kernel
+  int stages;    // units of K to a split
+  int64_t groups;  // workgroups of the main kernel
+  size_t bytes;    // workspace
+};
+
 struct Q4Args {
   const uint16_t* x;
   int64_t ldx;
@@ -47,6 +56,8 @@ struct Q4Args {
   int M, N, K, group;
   int out;  // llk_dtype
   int accumulate;
+  float* part;  // splits: [split][side][M][N] sums
+  int splits, stages;
 };
 
 hipError_t llk_launch_q4_pack(const Q4Source& s, uint8_t* codes, uint32_t* scales, hipStream_t stream);
@@ -59,4 +70,43 @@ struct Q4QuantiseArgs {
   int K, N, group, f16;
 };
 hipError_t llk_launch_q4_quantise(const Q4QuantiseArgs& a, hipStream_t stream);
-hipError_t llk_launch_q4(const Q4Args& a, int sides, hipStream_t stream);
+Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides);
+hipError_t llk_launch_q4(const Q4Args& a, int sides, const Q4Plan& plan, hipStream_t stream);
+hipError_t llk_launch_q4_tile(const Q4Args& a, int sides, int rows, hipStream_t stream);
+
+#ifdef __HIPCC__
+#include "common.h"
+
+namespace llk_gfx950 {
+
+constexpr uint32_t kCodeMask = 0x00780078u, kCodeOne = 0x3f803f80u;
+
+// A dword's 8 codes as bf16 1 + c / 16.
+__device__ __forceinline__ bf16x8 q4_decode8(uint32_t q) {
+  return __builtin_bit_cast(
+      bf16x8, u32x4{(q & kCodeMask) | kCodeOne, ((q >> 4) & kCodeMask) | kCodeOne,
+                    ((q >> 8) & kCodeMask) | kCodeOne,
+                    (__builtin_amdgcn_alignbit(q, q, 12) & kCodeMask) | kCodeOne});
+}
+__device__ __forceinline__ float q4_scale(uint32_t w) { return __uint_as_float(w & 0xffffe000u); }
+// -(1 + z / 16)
+__device__ __forceinline__ float q4_offset(uint32_t w) { return (float)(w & 0xffu) * -0.0625f; }
+
+// Results from the sums of (code - zero) / 16: times 16, SiLU(g) u, added to what is
+// there, rounded.
+__device__ __forceinline__ void q4_store(const Q4Args& a, int sides, int m, int n, float v, float u) {
+  const int64_t at = m * a.ldy + n;
+  float r = sides == 2 ? swiglu_act(v * 16.0f, u * 16.0f) : v * 16.0f;
+  if (a.out == kOutF32) {
+    float* const y = static_cast<float*>(a.y) + at;
+    *y = a.accumulate ? r + *y : r;
+  } else {
+    uint16_t* const y = static_cast<uint16_t*>(a.y) + at;
+    if (a.accumulate)
+      r += a.out == kOutBF16 ? bf16_bits_to_f32(*y) : (float)__builtin_bit_cast(_Float16, *y);
+    *y = a.out == kOutBF16 ? f32_to_bf16_rne(r) : f32_to_f16_rne(r);
+  }
+}
+
+}  // namespace llk_gfx950
+#endif

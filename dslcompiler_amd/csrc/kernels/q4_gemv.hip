@@ -22,25 +22,6 @@
 namespace llk_gfx950 {
 namespace {
 
-constexpr uint32_t kCodeMask = 0x00780078u, kCodeOne = 0x3f803f80u;
-
-__device__ __forceinline__ bf16x8 decode8(uint32_t q) {
-  return __builtin_bit_cast(
-      bf16x8, u32x4{(q & kCodeMask) | kCodeOne, ((q >> 4) & kCodeMask) | kCodeOne,
-                    ((q >> 8) & kCodeMask) | kCodeOne,
-                    (__builtin_amdgcn_alignbit(q, q, 12) & kCodeMask) | kCodeOne});
-}
-
-__device__ __forceinline__ float load_out(const Q4Args& a, int64_t at) {
-  if (a.out == kOutF32) return static_cast<const float*>(a.y)[at];
-  const uint16_t h = static_cast<const uint16_t*>(a.y)[at];
-  return a.out == kOutBF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-}
-__device__ __forceinline__ void store_out(const Q4Args& a, int64_t at, float v) {
-  if (a.out == kOutF32) static_cast<float*>(a.y)[at] = v;
-  else static_cast<uint16_t*>(a.y)[at] = a.out == kOutBF16 ? f32_to_bf16_rne(v) : f32_to_f16_rne(v);
-}
-
 // A wave's operands of one unit.
 template <int SIDES, int GROUP>
 struct Unit {
@@ -57,12 +38,12 @@ __global__ void __launch_bounds__(1024) q4_gemv_kernel(Q4Args a) {
   using U = Unit<SIDES, GROUP>;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int tile = blockIdx.x, m0 = blockIdx.y * 16, rows = min(16, a.M - m0);
+  const int tile = blockIdx.x, rows = a.M;  // to 16
   const int units = (a.K + kQ4Unit - 1) / kQ4Unit;
   const int col = lane & 15, grp = lane >> 4;
   // the lane's row of X: operand row col is row 4 (col % 4) + col / 4
   const int row = (col & 3) * 4 + (col >> 2);
-  const uint16_t* const x = a.x + (int64_t)(m0 + row) * a.ldx + grp * 8;
+  const uint16_t* const x = a.x + (int64_t)row * a.ldx + grp * 8;
 
   auto load = [&](int u, U& o) {
 #pragma unroll
@@ -111,13 +92,12 @@ __global__ void __launch_bounds__(1024) q4_gemv_kernel(Q4Args a) {
         sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs, ones, sx, 0, 0, 0);
 #pragma unroll
         for (int s = 0; s < SIDES; ++s)
-          part[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs, decode8(o.codes[s][j]), part[s], 0, 0, 0);
+          part[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs, q4_decode8(o.codes[s][j]), part[s], 0, 0, 0);
       }
 #pragma unroll
       for (int s = 0; s < SIDES; ++s) {
         const uint32_t w = o.scales[s][g];
-        const float scale = __uint_as_float(w & 0xffffe000u);
-        const float off = (float)(w & 0xffu) * -0.0625f;  // -(1 + z / 16)
+        const float scale = q4_scale(w), off = q4_offset(w);
 #pragma unroll
         for (int i = 0; i < MR; ++i)
           acc[s][i] = __builtin_fmaf(scale, __builtin_fmaf(off, sx[i], part[s][i]), acc[s][i]);
@@ -141,19 +121,15 @@ __global__ void __launch_bounds__(1024) q4_gemv_kernel(Q4Args a) {
       sums[((wave * SIDES + s) * MR * 4 + 4 * i + grp) * 16 + col] = acc[s][i];
   __syncthreads();
   for (int t = threadIdx.x; t < rows * 16; t += blockDim.x) {
-    const int m = m0 + t / 16, n = tile * kQ4Columns + t % 16;
+    const int m = t / 16, n = tile * kQ4Columns + t % 16;
     if (n >= a.N) continue;
     float v[SIDES];
 #pragma unroll
     for (int s = 0; s < SIDES; ++s) {
       v[s] = 0.0f;
       for (int w = 0; w < waves; ++w) v[s] += sums[(w * SIDES + s) * MR * 64 + t];
-      v[s] *= 16.0f;
     }
-    const int64_t at = m * a.ldy + n;
-    float r = SIDES == 2 ? swiglu_act(v[0], v[SIDES - 1]) : v[0];
-    if (a.accumulate) r += load_out(a, at);
-    store_out(a, at, r);
+    q4_store(a, SIDES, m, n, v[0], v[SIDES - 1]);
   }
 }
 
@@ -168,7 +144,7 @@ hipError_t launch(const Q4Args& args, hipStream_t stream) {
                    : mr == 2 ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 2>)
                    : mr == 3 ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 3>)
                              : reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 4>);
-  return hipLaunchKernel(fn, dim3((unsigned)q4_tiles(a.N), (a.M + 15) / 16), dim3(waves * 64), params,
+  return hipLaunchKernel(fn, dim3((unsigned)q4_tiles(a.N)), dim3(waves * 64), params,
                          (size_t)waves * SIDES * mr * 256, stream);
 }
 template <int SIDES>
@@ -181,7 +157,28 @@ hipError_t launch_group(const Q4Args& a, hipStream_t s) {
 }  // namespace
 }  // namespace llk_gfx950
 
-hipError_t llk_launch_q4(const Q4Args& a, int sides, hipStream_t stream) {
+// The kernel for 16 rows streams the weights once for them; the tile kernel shares
+// them among 32 or 64.
+Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
+  Q4Plan p{16, 1, (int)q4_units(K), q4_tiles(N), 0};
+  if (M <= 16) return p;
+  p.rows = M <= 32 ? 32 : 64;
+  const int64_t tiles = (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256);
+  const int64_t units = std::max<int64_t>(1, q4_units(K));
+  // two workgroups to a CU, at least 4 units to each
+  const int64_t s = std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, units / 4));
+  p.stages = (int)((units + s - 1) / s);
+  p.splits = (int)((units + p.stages - 1) / p.stages);
+  p.groups = tiles * p.splits;
+  p.bytes = p.splits > 1 ? (size_t)p.splits * sides * M * N * sizeof(float) : 0;
+  return p;
+}
+
+hipError_t llk_launch_q4(const Q4Args& args, int sides, const Q4Plan& plan, hipStream_t stream) {
   using namespace llk_gfx950;
+  Q4Args a = args;
+  a.splits = plan.splits;
+  a.stages = plan.stages;
+  if (plan.rows > 16) return llk_launch_q4_tile(a, sides, plan.rows, stream);
   return sides == 2 ? launch_group<2>(a, stream) : launch_group<1>(a, stream);
 }

@@ -1,0 +1,229 @@
+// q4_tile.hip -- products of more than 16 rows with 4-bit weights (q4.h): the
+// mathematics of q4_gemv.hip, 32 or 64 rows to a workgroup.
+//
+// Four waves share the rows, each with 64 columns of its own (32 of each side of a
+// SwiGLU), whose codes it takes from memory straight into operands, a unit of 128 k
+// ahead.  X goes through LDS in operand order, two buffers in turn, and with it the
+// sums of each row over a group, which the threads that move X add up on the way.
+#include <algorithm>
+
+#include "common.h"
+#include "q4.h"
+
+namespace llk_gfx950 {
+namespace {
+
+constexpr int kWaves = 4, kTiles = 4;  // column tiles of a wave
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Sum of 8 bf16.
+__device__ __forceinline__ float sum8(const u32x4& x) {
+  const bf16x2 one = __builtin_bit_cast(bf16x2, kCodeOne);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = x[i];  // (a bit cast of the element itself would take the first)
+    s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), one, s, false);
+  }
+  return s;
+}
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
+template <int SIDES, int GROUP, int RT>
+__global__ void __launch_bounds__(kWaves * 64)
+    __attribute__((amdgpu_waves_per_eu(2))) q4_tile_kernel(Q4Args a) {
+  constexpr int kRows = 16 * RT, kGroups = kQ4Unit / GROUP, kSteps = 4 / kGroups;
+  constexpr int kColumns = kWaves * kTiles * 16 / SIDES;  // of a side
+  // X: [step of 32 k][row tile][lane] of 16 bytes, a lane's place within its 16 turned
+  // by the chunk's number, so that the chunks of a row, which 16 threads write, meet
+  // different banks
+  __shared__ __attribute__((aligned(16))) u32x4 xs[2][4 * RT * 64];
+  __shared__ __attribute__((aligned(16))) float sums[2][kGroups][kRows];
+  const int t = threadIdx.x, lane = t & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int tiles_m = (a.M + kRows - 1) / kRows, tiles_n = (a.N + kColumns - 1) / kColumns;
+  const int id = xcd_remap(blockIdx.x, tiles_m * tiles_n * a.splits);
+  const int m0 = id % tiles_m * kRows, n0 = id / tiles_m % tiles_n * kColumns;
+  const int split = id / (tiles_m * tiles_n);
+  const int units = (a.K + kQ4Unit - 1) / kQ4Unit;
+  const int begin = split * a.stages, end = min(begin + a.stages, units);
+
+  // the wave's column tiles; past N its last one's again (not stored)
+  const int last = (a.N + 15) / 16 - 1;
+  int64_t tile[kTiles];
+#pragma unroll
+  for (int c = 0; c < kTiles; ++c)
+    tile[c] = (int64_t)min(n0 / 16 + wave * (kTiles / SIDES) + c % (kTiles / SIDES), last) * units;
+  struct Codes {
+    u32x4 q[kTiles];
+    uint32_t s[kTiles][kGroups];
+  };
+  auto load_codes = [&](int u, Codes& o) {
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) {
+      const Q4Side& side = a.side[c / (kTiles / SIDES)];
+      o.q[c] = reinterpret_cast<const u32x4*>(side.codes + (tile[c] + u) * kQ4UnitBytes)[lane];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        o.s[c][g] = side.scales[((tile[c] + u) * kGroups + g) * kQ4Columns + col];
+    }
+  };
+  // X: thread t moves chunk t % 16 (8 k) of rows t / 16 + 16 i; rows past M are the
+  // last one again
+  const int chunk = t & 15, xrow = t >> 4;
+  const uint16_t* xp[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+    xp[i] = a.x + (int64_t)min(m0 + xrow + 16 * i, a.M - 1) * a.ldx + 8 * chunk;
+  auto load_x = [&](int u, u32x4 (&x)[RT]) {
+    const int left = a.K - u * kQ4Unit - 8 * chunk;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const uint16_t* const p = xp[i] + (int64_t)u * kQ4Unit;
+      x[i] = left >= 8 ? load16_any(p) : load16_part(p, max(left, 0));
+    }
+  };
+  auto place_x = [&](int buf, const u32x4 (&x)[RT]) {
+    const int step = chunk >> 2, quarter = chunk & 3;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      xs[buf][(step * RT + i) * 64 + quarter * 16 + (xrow ^ chunk)] = x[i];
+      // over the 16 threads of the row, or 8 or 4 of them
+      float s = sum8(x[i]);
+      s = add_dpp<0xB1>(s);  // quad_perm: lane ^ 1
+      s = add_dpp<0x4E>(s);  // lane ^ 2
+      if constexpr (GROUP >= 64) s = add_dpp<0x141>(s);   // row_half_mirror
+      if constexpr (GROUP >= 128) s = add_dpp<0x140>(s);  // row_mirror
+      if (chunk % (GROUP / 8) == 0) sums[buf][chunk / (GROUP / 8)][xrow + 16 * i] = s;
+    }
+  };
+
+  f32x4 acc[RT][kTiles];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) acc[r][c] = f32x4{0, 0, 0, 0};
+  auto work = [&](int buf, const Codes& w) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      f32x4 part[RT][kTiles];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) part[r][c] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = g * kSteps; j < (g + 1) * kSteps; ++j) {
+        bf16x8 x[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          x[r] = __builtin_bit_cast(bf16x8, xs[buf][(j * RT + r) * 64 + grp * 16 + (col ^ (4 * j + grp))]);
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) {
+          const bf16x8 q = q4_decode8(w.q[c][j]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            part[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[r], q, part[r][c], 0, 0, 0);
+        }
+      }
+      f32x4 sx[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        sx[r] = *reinterpret_cast<const f32x4*>(&sums[buf][g][16 * r + 4 * grp]);
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) {
+        const float scale = q4_scale(w.s[c][g]), off = q4_offset(w.s[c][g]);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[r][c][i] =
+                __builtin_fmaf(scale, __builtin_fmaf(off, sx[r][i], part[r][c][i]), acc[r][c][i]);
+      }
+    }
+  };
+
+  Codes cur, next;
+  u32x4 x[RT];
+  if (begin < end) {
+    load_x(begin, x);
+    load_codes(begin, cur);
+  }
+  for (int u = begin; u < end; ++u) {
+    const int buf = (u - begin) & 1;
+    place_x(buf, x);  // its readers of two stages ago are past the barrier of the last
+    __syncthreads();
+    if (u + 1 < end) {
+      load_x(u + 1, x);
+      load_codes(u + 1, next);
+    }
+    work(buf, cur);
+    cur = next;
+  }
+
+  // lane: column col of each tile, rows 4 grp + i
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = m0 + 16 * r + 4 * grp + i;
+      if (m >= a.M) continue;
+#pragma unroll
+      for (int c = 0; c < kTiles / SIDES; ++c) {
+        const int n = n0 + (wave * (kTiles / SIDES) + c) * 16 + col;
+        if (n >= a.N) continue;
+        const float v = acc[r][c][i], w = acc[r][c + (SIDES - 1) * (kTiles / 2)][i];
+        if (a.splits == 1) {
+          q4_store(a, SIDES, m, n, v, w);
+        } else {
+          const int64_t plane = (int64_t)a.M * a.N, at = (int64_t)m * a.N + n;
+          a.part[split * SIDES * plane + at] = v;
+          if (SIDES == 2) a.part[(split * SIDES + 1) * plane + at] = w;
+        }
+      }
+    }
+}
+
+// Joins the splits in their order.
+template <int SIDES>
+__global__ void __launch_bounds__(256) q4_join_kernel(Q4Args a) {
+  const int64_t plane = (int64_t)a.M * a.N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
+    float v[2] = {};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+      for (int k = 0; k < SIDES; ++k) v[k] += a.part[(s * SIDES + k) * plane + i];
+    q4_store(a, SIDES, (int)(i / a.N), (int)(i % a.N), v[0], v[SIDES - 1]);
+  }
+}
+
+template <int SIDES, int RT>
+hipError_t launch(const Q4Args& args, hipStream_t stream) {
+  Q4Args a = args;
+  void* params[] = {&a};
+  const void* fn = a.group == 32   ? reinterpret_cast<const void*>(&q4_tile_kernel<SIDES, 32, RT>)
+                   : a.group == 64 ? reinterpret_cast<const void*>(&q4_tile_kernel<SIDES, 64, RT>)
+                                   : reinterpret_cast<const void*>(&q4_tile_kernel<SIDES, 128, RT>);
+  constexpr int kColumns = kWaves * kTiles * 16 / SIDES;
+  const int64_t groups = (int64_t)((a.M + 16 * RT - 1) / (16 * RT)) * ((a.N + kColumns - 1) / kColumns) *
+                         a.splits;
+  const hipError_t e =
+      hipLaunchKernel(fn, dim3((unsigned)groups), dim3(kWaves * 64), params, 0, stream);
+  if (e != hipSuccess || a.splits == 1) return e;
+  const int64_t all = ((int64_t)a.M * a.N + 255) / 256;
+  return hipLaunchKernel(reinterpret_cast<const void*>(&q4_join_kernel<SIDES>),
+                         dim3((unsigned)std::min<int64_t>(all, 1 << 16)), dim3(256), params, 0, stream);
+}
+
+}  // namespace
+}  // namespace llk_gfx950
+
+hipError_t llk_launch_q4_tile(const Q4Args& a, int sides, int rows, hipStream_t s) {
+  using namespace llk_gfx950;
+  if (sides == 2) return rows == 32 ? launch<2, 2>(a, s) : launch<2, 4>(a, s);
+  return rows == 32 ? launch<1, 2>(a, s) : launch<1, 4>(a, s);
+}

@@ -29,7 +29,7 @@ hipStream_t stream_of(const llk_kernel_context* ctx) {
 bool group_ok(int64_t g) { return g == 32 || g == 64 || g == 128; }
 // The packing kernels have a unit of K in a dimension of their grid (to 65535), and
 // indexes of 32 bits.
-constexpr int64_t kMaxK = (int64_t)65535 * 32, kMaxN = (int64_t)1 << 27;
+constexpr int64_t kMaxK = (int64_t)65535 * 32, kMaxN = (int64_t)1 << 26;
 
 int check_sizes(int64_t K, int64_t N, int64_t group) {
   if (!group_ok(group))
@@ -77,8 +77,9 @@ int check_packed(const llk_q4_weights* w, const char* name) {
   return LLK_OK;
 }
 
-// The rows of a launch: 16 to a workgroup, 65535 along a dimension.
-constexpr int64_t kMaxRows = (int64_t)65535 * 16;
+constexpr int64_t kMaxRows = (int64_t)1 << 24;
+// A dimension of a launch takes fewer than 2^32 threads: workgroups of 256.
+constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 1;
 
 int product(const llk_tensor2d* x, const llk_q4_weights* const (&w)[2], int sides, llk_tensor2d* y,
             int y_dtype, bool accumulate, llk_kernel_context* ctx) {
@@ -99,8 +100,6 @@ int product(const llk_tensor2d* x, const llk_q4_weights* const (&w)[2], int side
     return fail(LLK_ERR_DTYPE, "y type %d unsupported", y_dtype);
   if ((rc = check_matrix(y, "y", M, N, y_dtype == LLK_FP32 ? 4 : 2))) return rc;
   if (M == 0 || N == 0) return LLK_OK;
-  int dev;
-  if ((rc = llk::current_gfx950(&dev))) return rc;
   Q4Args a{};
   a.x = static_cast<const uint16_t*>(x->data);
   a.ldx = x->stride0;
@@ -115,7 +114,17 @@ int product(const llk_tensor2d* x, const llk_q4_weights* const (&w)[2], int side
   a.group = (int)w[0]->group;
   a.out = y_dtype;
   a.accumulate = accumulate;
-  const hipError_t e = llk_launch_q4(a, sides, stream_of(ctx));
+  const Q4Plan plan = llk_plan_q4(M, N, K, sides);
+  if (plan.groups > kMaxGroups)
+    return fail(LLK_ERR_SHAPE, "%lld rows of %lld columns are too many for one call", (long long)M,
+                (long long)N);
+  int dev;
+  if ((rc = llk::current_gfx950(&dev))) return rc;
+  llk::CallWorkspace ws;
+  if ((rc = ws.begin(dev, plan.bytes, ctx))) return rc;
+  a.part = static_cast<float*>(ws.ptr());
+  const hipError_t e = llk_launch_q4(a, sides, plan, stream_of(ctx));
+  ws.end();
   return e == hipSuccess ? LLK_OK : fail_hip(e, "4-bit product kernel");
 }
 
@@ -133,6 +142,12 @@ size_t llk_q4_scale_bytes(int64_t K, int64_t N, int64_t group) {
   return K < 0 || N < 0 || K > kMaxK || N > kMaxN || !group_ok(group)
              ? 0
              : (size_t)(q4_tiles(N) * q4_groups(K, (int)group)) * kQ4Columns * 4;
+}
+
+size_t llk_q4_scratch_size(int64_t M, int64_t N, int64_t K, int sides) {
+  return M < 0 || N < 0 || K < 0 || M > kMaxRows || K > kMaxK || N > kMaxN || sides < 1 || sides > 2
+             ? 0
+             : llk_plan_q4(M, N, K, sides).bytes;
 }
 
 int llk_q4_quantise(const llk_tensor2d* w, int64_t group, llk_tensor2d* codes, llk_tensor2d* scales,

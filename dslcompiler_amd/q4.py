@@ -106,7 +106,8 @@ def _packed(w, name: str, dev: int) -> _lib.Q4WeightsC:
     return w.c
 
 
-def q4_matmul(x, w: Q4Weights, *, out=None, out_dtype=None, accumulate: bool = False, stream=None):
+def q4_matmul(x, w: Q4Weights, *, out=None, out_dtype=None, accumulate: bool = False, stream=None,
+              scratch=None):
     """X W, x bf16 [M, K], to bf16, fp16 or fp32 (the default, as of matmul);
     with accumulate=True, out += X W, out being required.  Sums in fp32, weights
     as they are.  A row of X with an infinity or a NaN gives NaN."""
@@ -118,11 +119,13 @@ def q4_matmul(x, w: Q4Weights, *, out=None, out_dtype=None, accumulate: bool = F
             raise ValueError("accumulate=True needs `out`, the accumulator")
         out = x.new_empty((xd.dim0, w.N), dtype=out_dtype or _torch().float32)
     od, kind = _matrix(out, "out", dev, _OUT)
-    check(lib().llk_q4_gemm(xd, wc, od, kind, accumulate, _context(dev, stream)))
+    check(lib().llk_q4_gemm(xd, wc, od, kind, accumulate,
+                            _context(dev, stream, scratch)))
     return out
 
 
-def q4_swiglu(x, wg: Q4Weights, wu: Q4Weights, *, out=None, out_dtype=None, stream=None):
+def q4_swiglu(x, wg: Q4Weights, wu: Q4Weights, *, out=None, out_dtype=None, stream=None,
+              scratch=None):
     """SiLU(X Wg) * (X Wu), x bf16 [M, K], to bf16 (the default) or fp32; weights
     of one shape and group."""
     dev = _start()
@@ -131,5 +134,10 @@ def q4_swiglu(x, wg: Q4Weights, wu: Q4Weights, *, out=None, out_dtype=None, stre
     if out is None:
         out = x.new_empty((xd.dim0, wg.N), dtype=out_dtype or _torch().bfloat16)
     od, kind = _matrix(out, "out", dev, _SUMS)
-    check(lib().llk_q4_swiglu(xd, gc, uc, od, kind, _context(dev, stream)))
+    check(lib().llk_q4_swiglu(xd, gc, uc, od, kind, _context(dev, stream, scratch)))
     return out
+
+
+def q4_scratch_size(M: int, N: int, K: int, sides: int = 1) -> int:
+    """Bytes of `scratch` that q4_matmul (sides 1) and q4_swiglu (sides 2) need."""
+    return int(lib().llk_q4_scratch_size(M, N, K, sides))

@@ -560,6 +560,10 @@ int llk_q4_pack(const llk_tensor2d* codes, const llk_tensor2d* scales, int scale
 int llk_q4_gemm(const llk_tensor2d* x, const llk_q4_weights* w, llk_tensor2d* y, int y_dtype,
                 int accumulate, llk_kernel_context* ctx);
 
+/* ctx->scratch bytes that llk_q4_gemm (sides 1) and llk_q4_swiglu (sides 2) need
+ * where the caller supplies it (0: none).  Host only. */
+size_t llk_q4_scratch_size(int64_t M, int64_t N, int64_t K, int sides);
+
 /* Y = SiLU(X Wg) * (X Wu) on weights of one shape and group, y_dtype LLK_BF16 or
  * LLK_FP32; otherwise as llk_q4_gemm. */
 int llk_q4_swiglu(const llk_tensor2d* x, const llk_q4_weights* wg, const llk_q4_weights* wu,

@@ -48,7 +48,7 @@ def test_product_refusals(L):
     assert L.llk_q4_gemm(None, _w(), y, 0, 0, None) == -1
     assert L.llk_q4_gemm(x, _w(), None, 0, 0, None) == -1
     assert L.llk_q4_swiglu(x, _w(), None, y, 0, None) == -1
-    for bad, code in [(_t(4, 255), -2), (_t(-1, 256), -2), (_t(1 << 33, 256), -2),
+    for bad, code in [(_t(4, 255), -2), (_t(-1, 256), -2), (_t(1 << 25, 256), -2),
                       (_t(4, 256, stride=255), -4), (_t(4, 256, one=2), -4),
                       (_t(4, 256, data=FAKE + 1), -4), (_t(4, 256, data=None), -1)]:
         rows = bad.dim0
@@ -61,6 +61,13 @@ def test_product_refusals(L):
     assert L.llk_q4_swiglu(x, _w(), _w(), y, 1, None) == -3  # no fp16 result, as llk_swiglu_bf16
     assert L.llk_q4_swiglu(x, _w(), _w(N=32), y, 0, None) == -2
     assert L.llk_q4_swiglu(x, _w(), _w(group=128), y, 0, None) == -2
+    big = 1 << 24  # more workgroups than a launch takes
+    assert L.llk_q4_gemm(_t(big, 256), _w(N=1 << 16), _t(big, 1 << 16), 0, 0, None) == -2
+    assert b"too many" in L.llk_last_error()
+    assert L.llk_q4_scratch_size(16, 4096, 4096, 1) == 0
+    assert L.llk_q4_scratch_size(17, 4096, 4096, 1) % (17 * 4096 * 4) == 0
+    assert L.llk_q4_scratch_size(17, 16, 0, 2) == 0
+    assert L.llk_q4_scratch_size(-1, 4096, 4096, 1) == 0 and L.llk_q4_scratch_size(17, 16, 16, 3) == 0
     # nothing to do
     assert L.llk_q4_gemm(_t(0, 256), _w(), _t(0, 64), 0, 0, None) == 0
     assert L.llk_q4_gemm(x, _w(N=0), _t(4, 0), 0, 0, None) == 0
