@@ -41,6 +41,7 @@ struct Q4Side {
 // The launch of a product.
 struct Q4Plan {
   int rows;      // to a workgroup: 16 (the kernel for few rows), 32 or 64
+  int tiles;     // column tiles to a workgroup (the kernel for few rows)
   int splits;    // of K, joined by a second kernel
   int stages;    // units of K to a split
   int64_t groups;  // workgroups of the main kernel
@@ -58,6 +59,7 @@ struct Q4Args {
   int accumulate;
   float* part;  // splits: [split][side][M][N] sums
   int splits, stages;
+  int tiles;  // column tiles of the matrix
 };
 
 hipError_t llk_launch_q4_pack(const Q4Source& s, uint8_t* codes, uint32_t* scales, hipStream_t stream);
@@ -73,6 +75,7 @@ hipError_t llk_launch_q4_quantise(const Q4QuantiseArgs& a, hipStream_t stream);
 Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides);
 hipError_t llk_launch_q4(const Q4Args& a, int sides, const Q4Plan& plan, hipStream_t stream);
 hipError_t llk_launch_q4_tile(const Q4Args& a, int sides, int rows, hipStream_t stream);
+hipError_t llk_launch_q4_join(const Q4Args& a, int sides, hipStream_t stream);
 
 #ifdef __HIPCC__
 #include "common.h"

@@ -12,8 +12,11 @@
 // The columns are the lanes of the result (one scale to a lane), the rows 4 i + l /
 // 16 its register i, so up to 4 rows need one register of four.
 //
-// HBM bound: the waves of a workgroup take the units of a column tile in turn, and
-// join their sums in LDS.
+// HBM bound.  A workgroup has a few column tiles and a range of K: its rows of X go
+// to LDS once (read as operands from memory they are four times a unit's codes, and
+// the vector memory path, not HBM, would be the limit), and its 8 waves take the
+// range's units in turn, four of them on their way.  Their sums are joined in LDS, and
+// those of a split K by a second kernel.
 #include <algorithm>
 
 #include "common.h"
@@ -22,136 +25,168 @@
 namespace llk_gfx950 {
 namespace {
 
-// A wave's operands of one unit.
-template <int SIDES, int GROUP>
-struct Unit {
-  static constexpr int kGroups = kQ4Unit / GROUP;
-  u32x4 codes[SIDES];
-  uint32_t scales[SIDES][kGroups];
-  u32x4 x[4];
-};
+constexpr int kWaves = 8, kAhead = 4;
 
-// MR: registers of the result that hold rows (M <= 4 MR).
-template <int SIDES, int GROUP, int MR>
-__global__ void __launch_bounds__(1024) q4_gemv_kernel(Q4Args a) {
-  extern __shared__ float sums[];  // [wave][side][row][16]
-  using U = Unit<SIDES, GROUP>;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int tile = blockIdx.x, rows = a.M;  // to 16
+// MR: registers of the result that hold rows (M <= 4 MR).  C: column tiles.
+template <int SIDES, int GROUP, int MR, int C>
+__global__ void __launch_bounds__(kWaves * 64) q4_gemv_kernel(Q4Args a) {
+  // X: [unit][row][16 chunks of 8 k], a chunk's place turned by the row, so that 16
+  // rows' chunks meet all banks; then the waves' sums [wave][side][row][16]
+  extern __shared__ __attribute__((aligned(16))) u32x4 lds[];
+  constexpr int kGroups = kQ4Unit / GROUP, kTurns = kWaves / C;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = a.M;  // to 16
   const int units = (a.K + kQ4Unit - 1) / kQ4Unit;
-  const int col = lane & 15, grp = lane >> 4;
-  // the lane's row of X: operand row col is row 4 (col % 4) + col / 4
-  const int row = (col & 3) * 4 + (col >> 2);
-  const uint16_t* const x = a.x + (int64_t)row * a.ldx + grp * 8;
+  const int begin = blockIdx.y * a.stages, end = min(begin + a.stages, units);
+  const int tile0 = blockIdx.x * C, turn = wave / C;
+  // (past the last tile, the last again, not stored)
+  const int64_t tile = (int64_t)min(tile0 + wave % C, a.tiles - 1) * units;
 
-  auto load = [&](int u, U& o) {
+  // Codes and scales through buffers of the tile: units past its last read as zeros,
+  // without a branch that would have every load waited for.
+  struct Unit {
+    u32x4 codes[SIDES];
+    uint32_t scales[SIDES][kGroups];
+  };
+  __amdgpu_buffer_rsrc_t codes[SIDES], scales[SIDES];
+#pragma unroll
+  for (int s = 0; s < SIDES; ++s) {
+    codes[s] = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(a.side[s].codes + tile * kQ4UnitBytes), 0, units * kQ4UnitBytes, kBufferWord3);
+    scales[s] = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint32_t*>(a.side[s].scales + tile * kGroups * kQ4Columns), 0,
+        units * kGroups * kQ4Columns * 4, kBufferWord3);
+  }
+  auto load = [&](int u, Unit& o) {
 #pragma unroll
     for (int s = 0; s < SIDES; ++s) {
-      const int64_t at = (int64_t)tile * units + u;
-      o.codes[s] = __builtin_nontemporal_load(
-          reinterpret_cast<const u32x4*>(a.side[s].codes + at * kQ4UnitBytes) + lane);
+      // (2: not to stay in the caches; no other workgroup reads them)
+      o.codes[s] = __builtin_amdgcn_raw_buffer_load_b128(codes[s], u * kQ4UnitBytes + lane * 16, 0, 2);
 #pragma unroll
-      for (int g = 0; g < U::kGroups; ++g)
-        o.scales[s][g] = a.side[s].scales[(at * U::kGroups + g) * kQ4Columns + col];
+      for (int g = 0; g < kGroups; ++g)
+        o.scales[s][g] = __builtin_amdgcn_raw_buffer_load_b32(
+            scales[s], ((u * kGroups + g) * kQ4Columns + col) * 4, 0, 0);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o.x[j] = u32x4{0, 0, 0, 0};
-    if (row < rows) {
-      const int k = u * kQ4Unit + grp * 8;
-      if ((u + 1) * kQ4Unit <= a.K) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o.x[j] = load16_any(x + u * kQ4Unit + 32 * j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int left = a.K - (k + 32 * j);
-          if (left >= 8) o.x[j] = load16_any(x + u * kQ4Unit + 32 * j);
-          else if (left > 0) o.x[j] = load16_part(x + u * kQ4Unit + 32 * j, left);
-        }
-      }
-    }
+    __builtin_amdgcn_sched_barrier(0);  // in order, so that the oldest can be waited for
   };
+  Unit ring[kAhead];
+  const int first = begin + turn;
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) load(first + n * kTurns, ring[n]);
 
+  for (int i = threadIdx.x; i < (end - begin) * rows * 16; i += kWaves * 64) {
+    const int chunk = i & 15, m = (i >> 4) % rows, u = (i >> 4) / rows;
+    const int k = (begin + u) * kQ4Unit + 8 * chunk, left = a.K - k;
+    const uint16_t* const p = a.x + (int64_t)m * a.ldx + k;
+    lds[(u * rows + m) * 16 + (chunk ^ m)] = left >= 8 ? load16_any(p) : load16_part(p, max(left, 0));
+  }
+  __syncthreads();
+
+  // the lane's row of X: operand row col is row 4 (col % 4) + col / 4.  Rows past the
+  // last are the last again: no other row sees them, and they are not stored.
+  const int row = min((col & 3) * 4 + (col >> 2), rows - 1);
   float acc[SIDES][MR];
 #pragma unroll
   for (int s = 0; s < SIDES; ++s)
 #pragma unroll
     for (int i = 0; i < MR; ++i) acc[s][i] = 0.0f;
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{kCodeOne, kCodeOne, kCodeOne, kCodeOne});
-  auto work = [&](const U& o) {
-    constexpr int kSteps = 4 / U::kGroups;  // of 32 k, to a group
+  auto work = [&](int u, const Unit& o) {
+    constexpr int kSteps = 4 / kGroups;  // of 32 k, to a group
+    const u32x4* const xs = lds + ((u - begin) * rows + row) * 16;
 #pragma unroll
-    for (int g = 0; g < U::kGroups; ++g) {
+    for (int g = 0; g < kGroups; ++g) {
       f32x4 sx{0, 0, 0, 0}, part[SIDES];
 #pragma unroll
       for (int s = 0; s < SIDES; ++s) part[s] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int j = g * kSteps; j < (g + 1) * kSteps; ++j) {
-        const bf16x8 xs = __builtin_bit_cast(bf16x8, o.x[j]);
-        sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs, ones, sx, 0, 0, 0);
+        const bf16x8 x = __builtin_bit_cast(bf16x8, xs[(4 * j + grp) ^ row]);
+        sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, ones, sx, 0, 0, 0);
 #pragma unroll
         for (int s = 0; s < SIDES; ++s)
-          part[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs, q4_decode8(o.codes[s][j]), part[s], 0, 0, 0);
+          part[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, q4_decode8(o.codes[s][j]), part[s], 0, 0, 0);
       }
 #pragma unroll
       for (int s = 0; s < SIDES; ++s) {
-        const uint32_t w = o.scales[s][g];
-        const float scale = q4_scale(w), off = q4_offset(w);
+        const float scale = q4_scale(o.scales[s][g]), off = q4_offset(o.scales[s][g]);
 #pragma unroll
         for (int i = 0; i < MR; ++i)
           acc[s][i] = __builtin_fmaf(scale, __builtin_fmaf(off, sx[i], part[s][i]), acc[s][i]);
       }
     }
   };
-  if (wave < units) {
-    U cur, next;
-    load(wave, cur);
-    for (int u = wave; u < units; u += waves) {
-      if (u + waves < units) load(u + waves, next);
-      work(cur);
-      cur = next;
+  if (first < end) {
+    for (int u = first;;) {
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        work(u, ring[n]);
+        if ((u += kTurns) >= end) goto done;
+        __builtin_amdgcn_sched_barrier(0);
+        load(u + (kAhead - 1) * kTurns, ring[n]);
+      }
     }
   }
-
+done:
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int s = 0; s < SIDES; ++s)
 #pragma unroll
     for (int i = 0; i < MR; ++i)
       sums[((wave * SIDES + s) * MR * 4 + 4 * i + grp) * 16 + col] = acc[s][i];
   __syncthreads();
-  for (int t = threadIdx.x; t < rows * 16; t += blockDim.x) {
-    const int m = t / 16, n = tile * kQ4Columns + t % 16;
+  for (int t = threadIdx.x; t < rows * 16 * C; t += kWaves * 64) {
+    const int c = t / 16 % C, m = t / (16 * C), n = (tile0 + c) * kQ4Columns + t % 16;
     if (n >= a.N) continue;
     float v[SIDES];
 #pragma unroll
     for (int s = 0; s < SIDES; ++s) {
       v[s] = 0.0f;
-      for (int w = 0; w < waves; ++w) v[s] += sums[(w * SIDES + s) * MR * 64 + t];
+#pragma unroll
+      for (int w = 0; w < kTurns; ++w)
+        v[s] += sums[(((w * C + c) * SIDES + s) * MR * 4 + m) * 16 + t % 16];
     }
-    q4_store(a, SIDES, m, n, v[0], v[SIDES - 1]);
+    if (a.splits == 1) {
+      q4_store(a, SIDES, m, n, v[0], v[SIDES - 1]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < SIDES; ++s)
+        a.part[(int64_t)((blockIdx.y * SIDES + s) * a.M + m) * a.N + n] = v[s];
+    }
   }
 }
 
-template <int SIDES, int GROUP>
-hipError_t launch(const Q4Args& args, hipStream_t stream) {
+template <int SIDES, int GROUP, int MR>
+hipError_t launch(const Q4Args& args, const Q4Plan& plan, hipStream_t stream) {
   Q4Args a = args;
   void* params[] = {&a};
-  const int units = (int)q4_units(a.K);
-  const int waves = std::clamp(units, 1, 8);
-  const int mr = std::min(4, (a.M + 3) / 4);
-  const void* fn = mr == 1   ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 1>)
-                   : mr == 2 ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 2>)
-                   : mr == 3 ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 3>)
-                             : reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, 4>);
-  return hipLaunchKernel(fn, dim3((unsigned)q4_tiles(a.N)), dim3(waves * 64), params,
-                         (size_t)waves * SIDES * mr * 256, stream);
+  const void* fn = plan.tiles == 1   ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, MR, 1>)
+                   : plan.tiles == 2 ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, MR, 2>)
+                                     : reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, MR, 4>);
+  const size_t lds = std::max((size_t)a.stages * a.M * 256, (size_t)kWaves * SIDES * MR * 256);
+  // beyond 64 KiB, once per kernel and device
+  static std::atomic<uint64_t> set[3];
+  hipError_t e = hipSuccess;
+  if (lds > 65536) e = ensure_dynamic_lds(fn, 163840, set[plan.tiles / 2]);
+  if (e != hipSuccess) return e;
+  e = hipLaunchKernel(fn, dim3((unsigned)((a.tiles + plan.tiles - 1) / plan.tiles), (unsigned)a.splits),
+                      dim3(kWaves * 64), params, lds, stream);
+  return e != hipSuccess || a.splits == 1 ? e : llk_launch_q4_join(a, SIDES, stream);
+}
+template <int SIDES, int GROUP>
+hipError_t launch_rows(const Q4Args& a, const Q4Plan& p, hipStream_t s) {
+  return a.M <= 4    ? launch<SIDES, GROUP, 1>(a, p, s)
+         : a.M <= 8  ? launch<SIDES, GROUP, 2>(a, p, s)
+         : a.M <= 12 ? launch<SIDES, GROUP, 3>(a, p, s)
+                     : launch<SIDES, GROUP, 4>(a, p, s);
 }
 template <int SIDES>
-hipError_t launch_group(const Q4Args& a, hipStream_t s) {
-  return a.group == 32   ? launch<SIDES, 32>(a, s)
-         : a.group == 64 ? launch<SIDES, 64>(a, s)
-                         : launch<SIDES, 128>(a, s);
+hipError_t launch_group(const Q4Args& a, const Q4Plan& p, hipStream_t s) {
+  return a.group == 32   ? launch_rows<SIDES, 32>(a, p, s)
+         : a.group == 64 ? launch_rows<SIDES, 64>(a, p, s)
+                         : launch_rows<SIDES, 128>(a, p, s);
 }
 
 }  // namespace
@@ -160,16 +195,41 @@ hipError_t launch_group(const Q4Args& a, hipStream_t s) {
 // The kernel for 16 rows streams the weights once for them; the tile kernel shares
 // them among 32 or 64.
 Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
-  Q4Plan p{16, 1, (int)q4_units(K), q4_tiles(N), 0};
-  if (M <= 16) return p;
-  p.rows = M <= 32 ? 32 : 64;
-  const int64_t tiles = (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256);
   const int64_t units = std::max<int64_t>(1, q4_units(K));
-  // two workgroups to a CU, at least 4 units to each
-  const int64_t s = std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, units / 4));
+  Q4Plan p{};
+  int64_t s;  // splits of K  // splits
+  const int64_t columns = q4_tiles(N);
+  if (M <= 16) {
+    // A workgroup's X takes 256 M bytes a unit of K.  Without a split of K a call is one
+    // launch, about 3 us less than with the kernel that joins them; the columns are
+    // then a launch's only parallelism, so that few tiles go to a workgroup.  Measured,
+    // us, 1, 2 and 4 tiles: 4096 x 4096, 1 row, 4.7, 5.9, 8.4; 4096 x 14336, 9.6, 9.1,
+    // 9.5, SwiGLU 15.7, 15.1, 14.3.
+    p.rows = 16;
+    const bool two = sides == 2;
+    const int64_t x = M * units, four = (columns + 3) / 4;
+    if (x <= 256 || (x <= 640 && two && four >= 200)) {
+      // (640 is all of a CU's LDS: SwiGLU of 5120 x 13824, 16 rows, 26.7 us, split by 2
+      // 32.6, by 3 35.8)
+      p.tiles = two && columns >= 800 ? 4 : columns >= (two ? 400 : 640) ? 2 : 1;
+      s = 1;
+    } else {
+      // Two workgroups to a CU, 4 tiles each, at least 8 units.  13824 x 5120, 5 rows: 1
+      // tile, 1 split 18.4, 2 tiles, 3 splits 15.3, 4 tiles, 6 splits 15.2; 16 rows 30.5,
+      // 21.1 and 17.2.  4096 x 4096, 16 rows: 2 tiles, 2 splits 9.4, 4 and 4 8.5.
+      p.tiles = 4;
+      s = std::max((x + 319) / 320, std::min(480 / four, units / 8));
+    }
+  } else {
+    p.rows = M <= 32 ? 32 : 64;
+    const int64_t tiles = (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256);
+    // two workgroups to a CU, at least 4 units to each
+    s = std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, units / 4));
+  }
   p.stages = (int)((units + s - 1) / s);
   p.splits = (int)((units + p.stages - 1) / p.stages);
-  p.groups = tiles * p.splits;
+  p.groups = M <= 16 ? (q4_tiles(N) + p.tiles - 1) / p.tiles
+                     : (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256) * p.splits;
   p.bytes = p.splits > 1 ? (size_t)p.splits * sides * M * N * sizeof(float) : 0;
   return p;
 }
@@ -179,6 +239,7 @@ hipError_t llk_launch_q4(const Q4Args& args, int sides, const Q4Plan& plan, hipS
   Q4Args a = args;
   a.splits = plan.splits;
   a.stages = plan.stages;
+  a.tiles = (int)q4_tiles(a.N);
   if (plan.rows > 16) return llk_launch_q4_tile(a, sides, plan.rows, stream);
-  return sides == 2 ? launch_group<2>(a, stream) : launch_group<1>(a, stream);
+  return sides == 2 ? launch_group<2>(a, plan, stream) : launch_group<1>(a, plan, stream);
 }

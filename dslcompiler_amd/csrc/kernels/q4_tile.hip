@@ -213,14 +213,21 @@ hipError_t launch(const Q4Args& args, hipStream_t stream) {
                          a.splits;
   const hipError_t e =
       hipLaunchKernel(fn, dim3((unsigned)groups), dim3(kWaves * 64), params, 0, stream);
-  if (e != hipSuccess || a.splits == 1) return e;
-  const int64_t all = ((int64_t)a.M * a.N + 255) / 256;
-  return hipLaunchKernel(reinterpret_cast<const void*>(&q4_join_kernel<SIDES>),
-                         dim3((unsigned)std::min<int64_t>(all, 1 << 16)), dim3(256), params, 0, stream);
+  return e != hipSuccess || a.splits == 1 ? e : llk_launch_q4_join(a, SIDES, stream);
 }
 
 }  // namespace
 }  // namespace llk_gfx950
+
+hipError_t llk_launch_q4_join(const Q4Args& args, int sides, hipStream_t stream) {
+  using namespace llk_gfx950;
+  Q4Args a = args;
+  void* params[] = {&a};
+  const int64_t all = ((int64_t)a.M * a.N + 255) / 256;
+  return hipLaunchKernel(sides == 2 ? reinterpret_cast<const void*>(&q4_join_kernel<2>)
+                                    : reinterpret_cast<const void*>(&q4_join_kernel<1>),
+                         dim3((unsigned)std::min<int64_t>(all, 1 << 16)), dim3(256), params, 0, stream);
+}
 
 hipError_t llk_launch_q4_tile(const Q4Args& a, int sides, int rows, hipStream_t s) {
   using namespace llk_gfx950;

@@ -64,7 +64,8 @@ def test_product_refusals(L):
     big = 1 << 24  # more workgroups than a launch takes
     assert L.llk_q4_gemm(_t(big, 256), _w(N=1 << 16), _t(big, 1 << 16), 0, 0, None) == -2
     assert b"too many" in L.llk_last_error()
-    assert L.llk_q4_scratch_size(16, 4096, 4096, 1) == 0
+    assert L.llk_q4_scratch_size(1, 4096, 4096, 1) == 0
+    assert L.llk_q4_scratch_size(16, 4096, 13824, 1) % (16 * 4096 * 4) == 0
     assert L.llk_q4_scratch_size(17, 4096, 4096, 1) % (17 * 4096 * 4) == 0
     assert L.llk_q4_scratch_size(17, 16, 0, 2) == 0
     assert L.llk_q4_scratch_size(-1, 4096, 4096, 1) == 0 and L.llk_q4_scratch_size(17, 16, 16, 3) == 0
