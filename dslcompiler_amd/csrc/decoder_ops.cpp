@@ -284,10 +284,31 @@ int check_attention(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk
   return LLK_OK;
 }
 
-// Where the rows' statistics lie in the workspace of an attention that adds its
-// weights up: after the splits' parts.
-size_t stats_at(const AttentionPlan& p) { return (p.bytes + 255) / 256 * 256; }
-size_t stats_bytes(const llk_tensor3d* q) { return (size_t)(q->dim0 * q->dim1) * 2 * sizeof(float); }
+// The workspace of an attention that adds its weights up: the splits' parts, the rows'
+// statistics, and the scores of single tokens' rows.
+struct WeighPlan {
+  size_t stats, kept, bytes;  // where they begin; all
+  int kept_keys;              // of a sequence, or 0: none are kept
+};
+WeighPlan plan_weigh(const AttentionPlan& p, const Kv4AttentionArgs& a, const llk_tensor3d* q,
+                     int64_t max_len) {
+  WeighPlan w{};
+  w.stats = (p.bytes + 255) / 256 * 256;
+  w.kept = w.stats + ((size_t)(q->dim0 * q->dim1) * 2 * sizeof(float) + 255) / 256 * 256;
+  w.bytes = w.kept;
+  if (!a.batch.starts && p.rows == 16 && a.group <= 16) {
+    int64_t len = std::min<int64_t>((int64_t)a.batch.table_pages << a.cache.page_shift, kKv4MaxLength);
+    if (max_len > 0) len = std::min(len, max_len);
+    const int64_t keys = (len + 255) / 256 * 256;
+    const int64_t bytes = q->dim0 * q->dim1 * keys * (int64_t)sizeof(float);
+    // (a cache of as many keys takes 17/16 head_dim bytes for 4 group here)
+    if (keys > 0 && bytes <= (int64_t)512 << 20) {
+      w.kept_keys = (int)keys;
+      w.bytes += (size_t)bytes;
+    }
+  }
+  return w;
+}
 
 // The sequences' heads are workgroups of up to 1024 threads along one dimension.
 int check_heads(const Kv4Batch& b, int64_t heads) {
@@ -321,9 +342,14 @@ int attend(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk_kv4_batc
   int dev;
   if ((rc = llk::current_gfx950(&dev))) return rc;
   llk::CallWorkspace ws;
-  if ((rc = ws.begin(dev, marks ? stats_at(p) + stats_bytes(q) : p.bytes, ctx))) return rc;
+  const WeighPlan weigh = marks ? plan_weigh(p, a, q, batch->max_len) : WeighPlan{};
+  if ((rc = ws.begin(dev, marks ? weigh.bytes : p.bytes, ctx))) return rc;
   a.part = static_cast<float*>(ws.ptr());
-  if (marks) a.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(ws.ptr()) + stats_at(p));
+  if (marks) {
+    a.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(ws.ptr()) + weigh.stats);
+    a.kept_keys = weigh.kept_keys;
+    if (a.kept_keys) a.kept = reinterpret_cast<float*>(static_cast<uint8_t*>(ws.ptr()) + weigh.kept);
+  }
   hipError_t e = llk_launch_kv4_attention(a, (int)cache->head_dim, p.rows, stream_of(ctx));
   if (marks && e == hipSuccess)
     e = llk_launch_kv4_weigh(a, m, decay, (int)cache->head_dim, batch->max_len, stream_of(ctx));
@@ -479,10 +505,12 @@ int llk_kv4_attention_weigh_describe(const llk_tensor3d* q, const llk_kv4_cache*
                                      llk_attention_plan* out) {
   const int rc = llk_kv4_attention_describe(q, cache, batch, params, out);
   if (rc || out->launches == 0) return rc;
+  Kv4AttentionArgs a{};
   AttentionPlan p{};
-  p.bytes = out->workspace_bytes;
+  bool empty = false;
+  check_attention(q, cache, batch, params, &a, &p, &empty);
   out->launches += 1;
-  out->workspace_bytes = stats_at(p) + stats_bytes(q);
+  out->workspace_bytes = plan_weigh(p, a, q, batch->max_len).bytes;
   return LLK_OK;
 }
 

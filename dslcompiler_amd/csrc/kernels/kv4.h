@@ -63,6 +63,10 @@ struct Kv4AttentionArgs {
   int splits, chunk;  // splits of a sequence's key steps, steps to a split
   float scale;        // of q.k, times log2(e)
   float* stats;       // null, or [tokens][q heads][2]: a row's reference score and sum
+  // null, or the scores of single tokens' rows of 16 at most: [sequence][key head][row]
+  // [kept_keys], of the first kept_keys keys (a multiple of 256)
+  float* kept;
+  int kept_keys;
 };
 
 // A dimension of a launch takes fewer than 2^32 threads (with more it runs some of
@@ -92,7 +96,8 @@ hipError_t llk_launch_kv4_prompt(const Kv4AttentionArgs& a, int D, hipStream_t s
 hipError_t llk_launch_kv4_attention(const Kv4AttentionArgs& a, int D, int rows, hipStream_t s);
 size_t llk_kv4_attention_part_bytes(int64_t tiles, int heads, int splits, int rows, int D);
 
-// After an attention that left its rows' statistics: adds every key's weights up.
+// After an attention that left its rows' statistics, and their scores where it kept
+// them: adds every key's weights up.
 hipError_t llk_launch_kv4_weigh(const Kv4AttentionArgs& a, const Kv4Marks& marks, float decay, int D,
                                 int64_t max_len, hipStream_t s);
 

@@ -42,7 +42,8 @@ constexpr int kMinWaves =
 // 68 us, 5.3 TB/s; one token over 131072 keys (143 MB) 28 us, 5.1 TB/s, and 4 to
 // join the splits.  The codes of one row tile are read past the L2, since no
 // other workgroup reads them.
-template <int D, int RT>
+// KEEP: the scores are stored too, for the call that adds the weights up.
+template <int D, int RT, bool KEEP = false>
 __global__ void __launch_bounds__(kWaves * 64)
     __attribute__((amdgpu_waves_per_eu(kMinWaves<D, RT>))) kv4_attention_kernel(Kv4AttentionArgs a) {
   constexpr int R = 16 * RT, kD16 = D / 16, kJ = D / 32;
@@ -170,6 +171,14 @@ __global__ void __launch_bounds__(kWaves * 64)
 #pragma unroll
         for (int y = 0; y < RT; ++y)
           st[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[y][j], st[y][x], 0, 0, 0);
+      }
+    }
+
+    if constexpr (KEEP) {
+      if (col < a.group && k0 < a.kept_keys) {
+        float* const to = a.kept + ((int64_t)blockIdx.x * a.group + col) * a.kept_keys + k0 + 4 * grp;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) *reinterpret_cast<f32x4*>(to + 16 * x) = st[0][x];
       }
     }
 
@@ -356,7 +365,8 @@ hipError_t attend(const Kv4AttentionArgs& args, hipStream_t s) {
   Kv4AttentionArgs a = args;
   void* params[] = {&a};
   const hipError_t e = hipLaunchKernel(
-      reinterpret_cast<const void*>(&kv4_attention_kernel<D, RT>),
+      RT == 1 && a.kept ? reinterpret_cast<const void*>(&kv4_attention_kernel<D, 1, true>)
+                        : reinterpret_cast<const void*>(&kv4_attention_kernel<D, RT>),
       dim3((unsigned)(a.tiles * a.cache.heads), (unsigned)a.splits), dim3(kWaves * 64), params, 0, s);
   return e == hipSuccess && a.splits > 1 ? join<D, 16 * RT>(a, s) : e;
 }
