@@ -12,6 +12,7 @@
 // or rows are many, the scores are computed again: a prompt has far more pairs of a
 // row and a key than could be kept.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4_attention.h"
 
@@ -47,8 +48,9 @@ __device__ __forceinline__ float sum16(float x) {
 struct RowWeight {
   float shift, inv;  // exp2(score a.scale - shift) inv
   // nothing of a row that saw nothing, or scores of -infinity only
-  __device__ __forceinline__ RowWeight(const Kv4AttentionArgs& a, int64_t row, bool some) {
-    const float2 ml = reinterpret_cast<const float2*>(a.stats)[row];
+  __device__ __forceinline__ RowWeight(const Kv4AttentionArgs& a, int64_t row, bool some)
+      : RowWeight(a, reinterpret_cast<const float2*>(a.stats)[row], some) {}
+  __device__ __forceinline__ RowWeight(const Kv4AttentionArgs& a, float2 ml, bool some) {
     some = some && ml.y != 0.0f;
     shift = some ? ml.x * a.scale : 0.0f;
     inv = some ? 1.0f / ml.y : 0.0f;
@@ -179,29 +181,36 @@ __global__ void __launch_bounds__(kWaves * 64)
   }
 }
 
-// Many rows: a wave has 32 keys, in registers as operands, and meets all rows that
-// see them, 64 at a time in LDS, which the workgroup's four waves (128 keys) share.
-// S^T = K Q^T on v_mfma_f32_32x32x16_bf16, any order of the D values: of a key's, the
-// lane's half of the wave has the first or second half.
-constexpr int kKeys = 32, kQueries = 64;
+// Many rows: four waves share 128 keys, 32 of each, in registers as operands, four
+// more have the same keys, and the rows that see them go through LDS, 64 at a time,
+// half of them for either four.  S^T = K Q^T on v_mfma_f32_32x32x16_bf16, any order of
+// the D values: of a key's, the lane's half of the wave has the first or second half.
+//
+// What bounds it is LDS: every operand that is read meets one product.  A prompt of
+// 2048 tokens, 32 heads, takes 43 us (400 TFLOP/s of what causality leaves), 44
+// without the products or without the exponentials, and 38 with rows that stay in
+// LDS.  64 keys to a wave need more registers than there are (61 us).
+constexpr int kRowWaves = 8, kRowThreads = kRowWaves * 64, kRowKeys = 128;
 
 template <int D>
-__global__ void __launch_bounds__(kWaves * 64)
+__global__ void __launch_bounds__(kRowThreads)
     __attribute__((amdgpu_waves_per_eu(2))) kv4_weigh_rows_kernel(Kv4AttentionArgs a, Kv4Marks marks,
                                                                   float decay, int tiles) {
   constexpr int kU = D / 16, kBlocks = D / 64, kChunks = D / 8;
+  constexpr int kKeyWaves = kRowKeys / 32, kParts = kRowWaves / kKeyWaves;
+  constexpr int kQueries = 32 * kParts;  // rows to a round
   // Q: [32 rows][step u][half][row] of 16 bytes, a row's place turned by the chunk's
   // number, so that the chunks of a row meet different banks when they are written
-  __shared__ __attribute__((aligned(16))) u32x4 qs[2][kQueries / 32 * kU * 64];
+  __shared__ __attribute__((aligned(16))) u32x4 qs[2][kParts * kU * 64];
   __shared__ float2 weight[2][kQueries];  // shift, inv
   __shared__ int position[2][kQueries];
+  __shared__ float others[kParts][kRowKeys];  // the parts' sums
   const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  // The first tiles of keys, seen by the most rows, first, then the others from the
-  // last on, so that the two workgroups a CU gets in a round have much and little to do.
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6) % kKeyWaves;
+  const int part = __builtin_amdgcn_readfirstlane(t >> 6) / kKeyWaves;  // which 32 rows
+  // the first tiles of keys, seen by the most rows, first
   const int groups = a.batch.sequences * a.cache.heads;
-  const int nth = blockIdx.x / groups, head = blockIdx.x % groups % a.cache.heads;
-  const int tile = 2 * nth < tiles ? nth : tiles - 1 - (nth - (tiles + 1) / 2);
+  const int tile = blockIdx.x / groups, head = blockIdx.x % groups % a.cache.heads;
   Weighed w;
   if (!w.find(a, blockIdx.x % groups / a.cache.heads)) return;
   const int size = 1 << a.cache.page_shift;
@@ -209,15 +218,14 @@ __global__ void __launch_bounds__(kWaves * 64)
   const uint8_t* const base = a.cache.data + head * a.cache.head_bytes;
   const int heads = a.cache.heads * a.group;
 
-  for (int64_t first_key = (int64_t)tile * (kWaves * kKeys); first_key < w.len;
-       first_key += (int64_t)tiles * (kWaves * kKeys)) {
-    const int k0 = (int)first_key + wave * kKeys;  // the wave's keys
-    // the lane's key, its page, and its blocks
-    const int key = k0 + col, id = key < w.len ? table[key >> a.cache.page_shift] : -1;
-    const bool present = id >= 0 && id < a.cache.pages;
+  for (int64_t first_key = (int64_t)tile * kRowKeys; first_key < w.len;
+       first_key += (int64_t)tiles * kRowKeys) {
+    const int k0 = (int)first_key + wave * 32;  // the wave's keys
     bf16x8 k[kU];
     {
-      const uint8_t* const at = base + (present ? id : 0) * a.cache.page_stride +
+      // the lane's key, its page (0 without one; its sum is not stored), its blocks
+      const int key = k0 + col, id = key < w.len ? table[key >> a.cache.page_shift] : 0;
+      const uint8_t* const at = base + (id >= 0 && id < a.cache.pages ? id : 0) * a.cache.page_stride +
                                 ((key & (size - 1)) >> 4) * (17 * D);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
@@ -234,93 +242,141 @@ __global__ void __launch_bounds__(kWaves * 64)
 
     // rows of the first token that is not before the first key of the workgroup, to
     // the last that its window reaches
-    const int64_t from = (int64_t)max(0, (int)first_key - w.first) * a.group;
-    int64_t to = w.rows;
+    const int64_t seen_from = (int64_t)max(0, (int)first_key - w.first) * a.group;
+    int64_t seen_to = w.rows;
     if (a.window && first_key >= a.sinks)
-      to = min(to, max((int64_t)0, first_key + kWaves * kKeys - 1 + a.window - w.first) * a.group);
-    u32x4 x[kQueries * kChunks / 256];
+      seen_to = min(seen_to, max((int64_t)0, first_key + kRowKeys - 1 + a.window - w.first) * a.group);
+    const int from = (int)min(seen_from, seen_to), to = (int)seen_to;
+    // The thread's chunks are of kLoads rows, kRowThreads / kChunks apart, and one row's
+    // statistics.  Their addresses go from round to round by a constant, and by
+    // another where a row's query head passes the last (never, if a round's rows are a
+    // multiple of their number).
+    constexpr int kLoads = kQueries * kChunks / kRowThreads;
+    static_assert(kLoads * kRowThreads == kQueries * kChunks && kQueries <= kRowThreads, "rounds");
+    u32x4 x[kLoads];
     float2 ml;
     int at = 0;
-    auto row_at = [&](int64_t r) { return r < w.rows ? (int)r : w.rows - 1; };
-    auto load = [&](int64_t row0) {
+    const int tokens = kQueries / a.group, rest = kQueries % a.group;
+    const int last = w.rows - 1;
+    const uint16_t* const q =
+        a.q + w.token0 * a.q_token + (int64_t)head * a.group * a.q_head + t % kChunks * 8;
+    const float2* const stats =
+        reinterpret_cast<const float2*>(a.stats) + (int64_t)w.token0 * heads + head * a.group;
+    auto q_at = [&](int row) { return q + row / a.group * a.q_token + row % a.group * a.q_head; };
+    const int64_t q_step = tokens * a.q_token + rest * a.q_head, q_wrap = a.q_token - a.group * a.q_head;
+    const uint16_t* src[kLoads];
+    int q_head[kLoads];
 #pragma unroll
-      for (int i = 0; i < kQueries * kChunks / 256; ++i) {
-        const int n = i * 256 + t, row = row_at(row0 + n / kChunks);
-        const uint16_t* const src = a.q + (int64_t)(w.token0 + row / a.group) * a.q_token +
-                                    (int64_t)(head * a.group + row % a.group) * a.q_head;
-        x[i] = load16_any(src + n % kChunks * 8);
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = from + (i * kRowThreads + t) / kChunks;
+      src[i] = q_at(row);
+      q_head[i] = row % a.group;
+    }
+    const int own_row = from + t % kQueries;
+    int token = own_row / a.group, own_head = own_row % a.group;
+    auto load = [&](int row0) {
+      if (row0 >= to) return;
+      const bool whole = row0 + kQueries <= w.rows;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint16_t* p = src[i];
+        if (!whole && row0 + (i * kRowThreads + t) / kChunks > last) p = q_at(last);
+        x[i] = load16_any(p);
+        src[i] += q_step;
+        if (rest) {
+          q_head[i] += rest;
+          if (q_head[i] >= a.group) q_head[i] -= a.group, src[i] += q_wrap;
+        }
       }
       if (t < kQueries) {
-        const int row = row_at(row0 + t);
-        const bool some = row0 + t < w.rows;
-        const RowWeight r(a, (int64_t)(w.token0 + row / a.group) * heads + head * a.group + row % a.group,
-                          some);
-        ml = make_float2(r.shift, r.inv);
-        at = some ? w.first + row / a.group : kNowhere;
+        const bool some = row0 + t <= last;
+        ml = stats[some ? (int64_t)token * heads + own_head : 0];
+        at = some ? w.first + token : kNowhere;
+        token += tokens;
+        own_head += rest;
+        if (own_head >= a.group) own_head -= a.group, ++token;
       }
     };
     auto place = [&](int buf) {
 #pragma unroll
-      for (int i = 0; i < kQueries * kChunks / 256; ++i) {
-        const int n = i * 256 + t, q = n / kChunks, c = n % kChunks;  // chunk c: half c / kU, step c % kU
-        qs[buf][((q / 32 * kU + c % kU) * 2 + c / kU) * 32 + ((q ^ c) & 31)] = x[i];
+      for (int i = 0; i < kLoads; ++i) {
+        // row n, chunk c: half c / kU, step c % kU
+        const int n = (i * kRowThreads + t) / kChunks, c = t % kChunks;
+        qs[buf][((n / 32 * kU + c % kU) * 2 + c / kU) * 32 + ((n ^ c) & 31)] = x[i];
       }
-      if (t < kQueries) weight[buf][t] = ml, position[buf][t] = at;
+      if (t < kQueries) {  // (only here, so that the load before is not waited for at once)
+        const RowWeight r(a, ml, at != kNowhere);
+        weight[buf][t] = make_float2(r.shift, r.inv);
+        position[buf][t] = at;
+      }
     };
-    __syncthreads();  // the last reads of the tile of keys before
-    if (from < to) load(from);
-    int buf = 0;
-    for (int64_t row0 = from; row0 < to; row0 += kQueries, buf ^= 1) {
+    int p_lo = w.first + from / a.group, lo_head = from % a.group;  // of a round's first row
+    auto round = [&](int row0, auto which) {
+      constexpr int buf = decltype(which)::value;
       place(buf);  // its readers of two rounds ago are past the barrier of the last
       __syncthreads();
-      if (row0 + kQueries < to) load(row0 + kQueries);
-      // every row sees every key of the wave
-      const int p_lo = w.first + (int)(row0 / a.group);
-      const int p_hi = w.first + (int)(min(row0 + kQueries, (int64_t)w.rows) - 1) / a.group;
-      const bool whole = row0 + kQueries <= w.rows && k0 + kKeys - 1 <= p_lo &&
-                         (!a.window || k0 > p_hi - a.window || k0 + kKeys <= a.sinks);
-      if (k0 > p_hi) continue;  // none does
+      load(row0 + kQueries);
+      const int p_hi = p_lo + (lo_head + kQueries - 1) / a.group;  // (rows past the last: more)
+      const int p_first = row0 + kQueries <= w.rows ? p_lo : kNowhere;
+      p_lo += tokens;
+      lo_head += rest;
+      if (lo_head >= a.group) lo_head -= a.group, ++p_lo;
+      // (all operands are asked for before the first product: left to itself the
+      // compiler reads each where it is used and waits for it)
+      bf16x8 o[kU];
 #pragma unroll
-      for (int h = 0; h < kQueries / 32; ++h) {
-        f32x16 st;
+      for (int u = 0; u < kU; ++u)
+        o[u] = __builtin_bit_cast(
+            bf16x8, qs[buf][((part * kU + u) * 2 + half) * 32 + ((col ^ (half * kU + u)) & 31)]);
+      const float2 r = weight[buf][32 * part + col];
+      const int pos = position[buf][32 * part + col];
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 st;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = 0.0f;
+      for (int i = 0; i < 16; ++i) st[i] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int c = half * kU + u;
-          st = mfma32(k[u],
-                      __builtin_bit_cast(bf16x8, qs[buf][((h * kU + u) * 2 + half) * 32 + ((col ^ c) & 31)]),
-                      st);
-        }
-        const float2 r = weight[buf][32 * h + col];
-        if (whole) {
+      for (int u = 0; u < kU; ++u) st = mfma32(k[u], o[u], st);
+      // every row sees every key
+      if (k0 + 31 <= p_first && (!a.window || k0 > p_hi - a.window || k0 + 32 <= a.sinks)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sum[i] = __builtin_fmaf(
-                __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale, -r.x)), r.y, sum[i]);
-        } else {
-          const int pos = position[buf][32 * h + col];
+        for (int i = 0; i < 16; ++i)
+          sum[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale, -r.x)), r.y,
+                                  sum[i]);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale, -r.x)) * r.y;
-            sum[i] += sees(a, pos, k0 + 8 * (i >> 2) + 4 * half + (i & 3)) ? e : 0.0f;
-          }
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale, -r.x)) * r.y;
+          sum[i] += sees(a, pos, k0 + 8 * (i >> 2) + 4 * half + (i & 3)) ? e : 0.0f;
         }
       }
+    };
+    __syncthreads();  // the last reads of the tile of keys before
+    load(from);
+    for (int row0 = from; row0 < to; row0 += 2 * kQueries) {
+      round(row0, std::integral_constant<int, 0>{});
+      if (row0 + kQueries < to) round(row0 + kQueries, std::integral_constant<int, 1>{});
     }
-    // over the 32 lanes of a half wave; lane n stores the sum of its half's key n
-    float mine = 0.0f;
+
+    // over the 32 lanes of a half wave, then the parts; lane n has its half's key n
+    float own_sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float s = sum16(sum[i]);
       s += __shfl_xor(s, 16);
-      mine = col == i ? s : mine;
+      own_sum = col == i ? s : own_sum;
     }
-    const int own = k0 + 8 * (col >> 2) + 4 * half + (col & 3);  // of lanes col < 16
-    const int page = __shfl(present ? id : -1, own - k0 & 31);
-    if (col < 16 && own < w.len && page >= 0)
-      add_weight(marks.weights + page * marks.weights_page + (int64_t)head * size + (own & (size - 1)),
-                 decay, mine);
+    if (col < 16) others[part][wave * 32 + 8 * (col >> 2) + 4 * half + (col & 3)] = own_sum;
+    __syncthreads();
+    if (t < kRowKeys) {
+      const int64_t key = first_key + t;
+      float all = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) all += others[n][t];
+      const int id = key < w.len ? table[key >> a.cache.page_shift] : -1;
+      if (id >= 0 && id < a.cache.pages)
+        add_weight(marks.weights + id * marks.weights_page + (int64_t)head * size + (key & (size - 1)),
+                   decay, all);
+    }
   }
 }
 
@@ -338,13 +394,12 @@ hipError_t llk_launch_kv4_weigh(const Kv4AttentionArgs& args, const Kv4Marks& m,
   const int64_t groups = (int64_t)a.batch.sequences * a.cache.heads;
   if (!a.kept && (int64_t)a.batch.tokens * a.group > 16 * (int64_t)a.batch.sequences) {
     // (fewer workgroups go round for the rest)
-    int tiles = (int)std::min<int64_t>((len + kWaves * kKeys - 1) / (kWaves * kKeys),
-                                       kKv4MaxWorkgroups / groups);
+    int tiles = (int)std::min<int64_t>((len + kRowKeys - 1) / kRowKeys, kKv4MaxWorkgroups / 2 / groups);
     void* params[] = {&a, &marks, &decay, &tiles};
     const void* fn = D == 64    ? reinterpret_cast<const void*>(&kv4_weigh_rows_kernel<64>)
                      : D == 128 ? reinterpret_cast<const void*>(&kv4_weigh_rows_kernel<128>)
                                 : reinterpret_cast<const void*>(&kv4_weigh_rows_kernel<256>);
-    return hipLaunchKernel(fn, dim3((unsigned)(groups * tiles)), dim3(kWaves * 64), params, 0, s);
+    return hipLaunchKernel(fn, dim3((unsigned)(groups * tiles)), dim3(kRowThreads), params, 0, s);
   }
   const int64_t all = (len + kStep - 1) / kStep;  // steps of a sequence, at most
   // about 8192 waves; with kept scores 256 keys to a wave
