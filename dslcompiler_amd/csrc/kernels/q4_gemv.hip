@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_gemv_kernel(Q4Args a) {
   constexpr int kGroups = kQ4Unit / GROUP, kTurns = kWaves / C;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rows = a.M;  // to 16
+  const int m0 = blockIdx.z * 16, rows = min(16, a.M - m0);
   const int units = (a.K + kQ4Unit - 1) / kQ4Unit;
   const int begin = blockIdx.y * a.stages, end = min(begin + a.stages, units);
   const int tile0 = blockIdx.x * C, turn = wave / C;
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_gemv_kernel(Q4Args a) {
   for (int i = threadIdx.x; i < (end - begin) * rows * 16; i += kWaves * 64) {
     const int chunk = i & 15, m = (i >> 4) % rows, u = (i >> 4) / rows;
     const int k = (begin + u) * kQ4Unit + 8 * chunk, left = a.K - k;
-    const uint16_t* const p = a.x + (int64_t)m * a.ldx + k;
+    const uint16_t* const p = a.x + (int64_t)(m0 + m) * a.ldx + k;
     lds[(u * rows + m) * 16 + (chunk ^ m)] = left >= 8 ? load16_any(p) : load16_part(p, max(left, 0));
   }
   __syncthreads();
@@ -149,8 +149,8 @@ done:
         v[s] += sums[(((w * C + c) * SIDES + s) * MR * 4 + m) * 16 + t % 16];
     }
     if (a.splits == 1) {
-      q4_store(a, SIDES, m, n, v[0], v[SIDES - 1]);
-    } else {
+      q4_store(a, SIDES, m0 + m, n, v[0], v[SIDES - 1]);
+    } else {  // (one group of rows)
 #pragma unroll
       for (int s = 0; s < SIDES; ++s)
         a.part[(int64_t)((blockIdx.y * SIDES + s) * a.M + m) * a.N + n] = v[s];
@@ -165,13 +165,15 @@ hipError_t launch(const Q4Args& args, const Q4Plan& plan, hipStream_t stream) {
   const void* fn = plan.tiles == 1   ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, MR, 1>)
                    : plan.tiles == 2 ? reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, MR, 2>)
                                      : reinterpret_cast<const void*>(&q4_gemv_kernel<SIDES, GROUP, MR, 4>);
-  const size_t lds = std::max((size_t)a.stages * a.M * 256, (size_t)kWaves * SIDES * MR * 256);
+  const size_t lds =
+      std::max((size_t)a.stages * std::min(a.M, 16) * 256, (size_t)kWaves * SIDES * MR * 256);
   // beyond 64 KiB, once per kernel and device
   static std::atomic<uint64_t> set[3];
   hipError_t e = hipSuccess;
   if (lds > 65536) e = ensure_dynamic_lds(fn, 163840, set[plan.tiles / 2]);
   if (e != hipSuccess) return e;
-  e = hipLaunchKernel(fn, dim3((unsigned)((a.tiles + plan.tiles - 1) / plan.tiles), (unsigned)a.splits),
+  e = hipLaunchKernel(fn, dim3((unsigned)((a.tiles + plan.tiles - 1) / plan.tiles), (unsigned)a.splits,
+                           (unsigned)((a.M + 15) / 16)),
                       dim3(kWaves * 64), params, lds, stream);
   return e != hipSuccess || a.splits == 1 ? e : llk_launch_q4_join(a, SIDES, stream);
 }
@@ -199,7 +201,7 @@ Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
   Q4Plan p{};
   int64_t s;  // splits of K  // splits
   const int64_t columns = q4_tiles(N);
-  if (M <= 16) {
+  if (M <= 16 || K < 8) {  // (the tile kernel reads 8 elements of a row at once)
     // A workgroup's X takes 256 M bytes a unit of K.  Without a split of K a call is one
     // launch, about 3 us less than with the kernel that joins them; the columns are
     // then a launch's only parallelism, so that few tiles go to a workgroup.  Measured,
@@ -207,7 +209,7 @@ Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
     // 9.5, SwiGLU 15.7, 15.1, 14.3.
     p.rows = 16;
     const bool two = sides == 2;
-    const int64_t x = M * units, four = (columns + 3) / 4;
+    const int64_t x = std::min<int64_t>(M, 16) * units, four = (columns + 3) / 4;
     if (x <= 256 || (x <= 640 && two && four >= 200)) {
       // (640 is all of a CU's LDS: SwiGLU of 5120 x 13824, 16 rows, 26.7 us, split by 2
       // 32.6, by 3 35.8)
@@ -228,8 +230,8 @@ Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
   }
   p.stages = (int)((units + s - 1) / s);
   p.splits = (int)((units + p.stages - 1) / p.stages);
-  p.groups = M <= 16 ? (q4_tiles(N) + p.tiles - 1) / p.tiles
-                     : (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256) * p.splits;
+  p.groups = p.rows == 16 ? std::max((columns + p.tiles - 1) / p.tiles, (M + 15) / 16 * 256)
+                          : (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256) * p.splits;
   p.bytes = p.splits > 1 ? (size_t)p.splits * sides * M * N * sizeof(float) : 0;
   return p;
 }

@@ -52,12 +52,21 @@ __global__ void __launch_bounds__(kWaves * 64)
   const int units = (a.K + kQ4Unit - 1) / kQ4Unit;
   const int begin = split * a.stages, end = min(begin + a.stages, units);
 
-  // the wave's column tiles; past N its last one's again (not stored)
-  const int last = (a.N + 15) / 16 - 1;
-  int64_t tile[kTiles];
+  // The wave's column tiles; past N its last one's again (not stored).  Codes and
+  // scales through buffers of the tiles: units past their last read as zeros, without
+  // a branch that would have every load waited for.
+  __amdgpu_buffer_rsrc_t codes[kTiles], scales[kTiles];
 #pragma unroll
-  for (int c = 0; c < kTiles; ++c)
-    tile[c] = (int64_t)min(n0 / 16 + wave * (kTiles / SIDES) + c % (kTiles / SIDES), last) * units;
+  for (int c = 0; c < kTiles; ++c) {
+    const Q4Side& side = a.side[c / (kTiles / SIDES)];
+    const int64_t tile =
+        (int64_t)min(n0 / 16 + wave * (kTiles / SIDES) + c % (kTiles / SIDES), a.tiles - 1) * units;
+    codes[c] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(side.codes + tile * kQ4UnitBytes),
+                                                 0, units * kQ4UnitBytes, kBufferWord3);
+    scales[c] = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint32_t*>(side.scales + tile * kGroups * kQ4Columns), 0,
+        units * kGroups * kQ4Columns * 4, kBufferWord3);
+  }
   struct Codes {
     u32x4 q[kTiles];
     uint32_t s[kTiles][kGroups];
@@ -65,26 +74,35 @@ __global__ void __launch_bounds__(kWaves * 64)
   auto load_codes = [&](int u, Codes& o) {
 #pragma unroll
     for (int c = 0; c < kTiles; ++c) {
-      const Q4Side& side = a.side[c / (kTiles / SIDES)];
-      o.q[c] = reinterpret_cast<const u32x4*>(side.codes + (tile[c] + u) * kQ4UnitBytes)[lane];
+      o.q[c] = __builtin_amdgcn_raw_buffer_load_b128(codes[c], u * kQ4UnitBytes + lane * 16, 0, 0);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        o.s[c][g] = side.scales[((tile[c] + u) * kGroups + g) * kQ4Columns + col];
+        o.s[c][g] = __builtin_amdgcn_raw_buffer_load_b32(
+            scales[c], ((u * kGroups + g) * kQ4Columns + col) * 4, 0, 0);
     }
   };
   // X: thread t moves chunk t % 16 (8 k) of rows t / 16 + 16 i; rows past M are the
-  // last one again
+  // last one again.  A chunk past K is read where K ends, and put right as it is placed.
   const int chunk = t & 15, xrow = t >> 4;
   const uint16_t* xp[RT];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-    xp[i] = a.x + (int64_t)min(m0 + xrow + 16 * i, a.M - 1) * a.ldx + 8 * chunk;
-  auto load_x = [&](int u, u32x4 (&x)[RT]) {
-    const int left = a.K - u * kQ4Unit - 8 * chunk;
+  for (int i = 0; i < RT; ++i) xp[i] = a.x + (int64_t)min(m0 + xrow + 16 * i, a.M - 1) * a.ldx;
+  auto load_x = [&](int u, u32x4 (&x)[RT]) {  // (K >= 8)
+    const int at = min(u * kQ4Unit + 8 * chunk, a.K - 8);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) x[i] = load16_any(xp[i] + at);
+  };
+  auto end_x = [&](int u, u32x4 (&x)[RT]) {  // of the unit that K ends in
+    const int past = u * kQ4Unit + 8 * chunk - (a.K - 8);  // elements
+    if (past <= 0) return;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const uint16_t* const p = xp[i] + (int64_t)u * kQ4Unit;
-      x[i] = left >= 8 ? load16_any(p) : load16_part(p, max(left, 0));
+      u32x4 v = past >= 8 ? u32x4{0, 0, 0, 0} : x[i];
+      if (past & 4) v = u32x4{v[2], v[3], 0, 0};
+      if (past & 2) v = u32x4{v[1], v[2], v[3], 0};
+      if (past & 1)
+        v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+      x[i] = v;
     }
   };
   auto place_x = [&](int buf, const u32x4 (&x)[RT]) {
@@ -146,22 +164,27 @@ __global__ void __launch_bounds__(kWaves * 64)
     }
   };
 
-  Codes cur, next;
+  Codes even, odd;
   u32x4 x[RT];
-  if (begin < end) {
-    load_x(begin, x);
-    load_codes(begin, cur);
-  }
-  for (int u = begin; u < end; ++u) {
-    const int buf = (u - begin) & 1;
-    place_x(buf, x);  // its readers of two stages ago are past the barrier of the last
+  load_x(begin, x);
+  __builtin_amdgcn_sched_barrier(0);  // loads in order, so that the oldest can be waited for
+  load_codes(begin, even);
+  // (two units to a turn: no loaded register is copied, which would wait for it)
+  auto unit = [&](int u, int buf, const Codes& now, Codes& next) {
+    if ((u + 1) * kQ4Unit > a.K) end_x(u, x);
+    place_x(buf, x);  // its readers of two units ago are past the barrier of the last
     __syncthreads();
-    if (u + 1 < end) {
-      load_x(u + 1, x);
-      load_codes(u + 1, next);
-    }
-    work(buf, cur);
-    cur = next;
+    load_x(u + 1, x);
+    __builtin_amdgcn_sched_barrier(0);
+    load_codes(u + 1, next);
+    __builtin_amdgcn_sched_barrier(0);
+    work(buf, now);
+  };
+  for (int u = begin;;) {
+    unit(u, 0, even, odd);
+    if (++u == end) break;
+    unit(u, 1, odd, even);
+    if (++u == end) break;
   }
 
   // lane: column col of each tile, rows 4 grp + i
