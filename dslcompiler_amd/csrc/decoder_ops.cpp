@@ -286,6 +286,7 @@ int check_attention(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk
 
 // The workspace of an attention that adds its weights up: the splits' parts, the rows'
 // statistics, and the scores of single tokens' rows.
+constexpr int64_t kMaxKept = (int64_t)512 << 20;  // bytes of scores
 struct WeighPlan {
   size_t stats, kept, bytes;  // where they begin; all
   int kept_keys;              // of a sequence, or 0: none are kept
@@ -300,9 +301,9 @@ WeighPlan plan_weigh(const AttentionPlan& p, const Kv4AttentionArgs& a, const ll
     int64_t len = std::min<int64_t>((int64_t)a.batch.table_pages << a.cache.page_shift, kKv4MaxLength);
     if (max_len > 0) len = std::min(len, max_len);
     const int64_t keys = (len + 255) / 256 * 256;
-    const int64_t bytes = q->dim0 * q->dim1 * keys * (int64_t)sizeof(float);
-    // (a cache of as many keys takes 17/16 head_dim bytes for 4 group here)
-    if (keys > 0 && bytes <= (int64_t)512 << 20) {
+    const double bytes = (double)(q->dim0 * q->dim1) * (double)keys * sizeof(float);
+    // (4 group bytes for a key and head, of which the cache has 17/16 head_dim)
+    if (keys > 0 && bytes <= (double)kMaxKept) {
       w.kept_keys = (int)keys;
       w.bytes += (size_t)bytes;
     }

@@ -202,23 +202,22 @@ def kv4_marks(pages: int, heads: int, page_size: int, device="cuda"):
             torch.zeros(shape, dtype=torch.int32, device=device))
 
 
+def _mark(t, name: str, shape, kinds, dev: int) -> tuple:
+    """(address, page stride) of one of a cache's marks; shape: (pages, heads,
+    page_size)."""
+    _kind(t, name, dev, kinds)
+    if t.shape != shape:
+        raise ValueError(f"{name} must be [pages, heads, page_size] = {list(shape)}")
+    step, head, one = t.stride()
+    if (shape[2] > 1 and one != 1) or (shape[1] > 1 and head != shape[2]):
+        raise ValueError(f"the heads of a page of {name} must be contiguous")
+    return t.data_ptr(), step
+
+
 def _marks(weights, positions, shape, dev: int) -> _lib.Kv4Marks:
-    """shape: (pages, heads, page_size) of the cache, or None: of the marks."""
-    c = _lib.Kv4Marks(None, None, 0, 0)
-    for name, t, kinds in (("weights", weights, _FP32), ("positions", positions, _INT32)):
-        if t is None:
-            continue
-        _kind(t, name, dev, kinds)
-        if t.dim() != 3 or tuple(t.shape) != (shape or tuple(t.shape)):
-            raise ValueError(f"{name} must be [pages, heads, page_size]" +
-                             (f" = {shape}" if shape else ""))
-        shape = tuple(t.shape)
-        step, head, one = t.stride()
-        if (shape[2] > 1 and one != 1) or (shape[1] > 1 and head != shape[2]):
-            raise ValueError(f"the heads of a page of {name} must be contiguous")
-        setattr(c, name, t.data_ptr())
-        setattr(c, name + "_stride", step)
-    return c
+    w, ws = (None, 0) if weights is None else _mark(weights, "weights", shape, _FP32, dev)
+    p, ps = (None, 0) if positions is None else _mark(positions, "positions", shape, _INT32, dev)
+    return _lib.Kv4Marks(w, p, ws, ps)
 
 
 def kv4_write(k, v, cache, table, lens, *, starts=None, weights=None, positions=None, at=None,
@@ -329,19 +328,19 @@ def kv4_evict_plan(weights, table, lens, keep: int, *, positions=None, recent: i
     those from keep on that stay, both in order.  Nothing is moved, and lens stays
     as it is (lens_out must be other memory)."""
     dev = _begin()
-    marks = _marks(weights, positions, None, dev)
-    if weights is None:
-        raise ValueError("weights is required")
-    batch = _batch(table, lens, None, lens.shape[0], max_len, dev)
-    torch = _torch()
-    pages, heads, size = weights.shape
+    _kind(weights, "weights", dev, _FP32)
+    if weights.dim() != 3:
+        raise ValueError("weights must be [pages, heads, page_size]")
+    pages, heads, size = shape = weights.shape
+    marks = _marks(weights, positions, shape, dev)
+    batch = _batch(table, lens, None, table.shape[0], max_len, dev)
     if lens_out is None:
-        lens_out = torch.empty(lens.shape, dtype=torch.int32, device=lens.device)
+        lens_out = lens.new_empty(lens.shape)
     else:
         _kind(lens_out, "lens_out", dev, _INT32)
         if lens_out.shape != lens.shape or (lens.shape[0] > 1 and lens_out.stride(0) != 1):
             raise ValueError("lens_out must be a contiguous vector like lens")
-    source = torch.empty((lens.shape[0], heads, max(keep, 0)), dtype=torch.int32, device=lens.device)
+    source = lens.new_empty((batch.sequences, heads, max(keep, 0)))
     check(lib().llk_kv4_evict_plan(marks, pages, heads, size, batch,
                                    _lib.EvictParams(keep, recent, first), lens_out.data_ptr(),
                                    source.data_ptr(), _context(dev, stream)))

@@ -10,7 +10,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import LLK_BF16, LLK_FP32, check, lib
-from .decoder import _begin, _context, _kind, _result
+from .decoder import _begin, _context, _kind
 from .ops import _torch
 
 _SCALINGS = {None: 0, "linear": 1, "base": 2, "yarn": 3, "bands": 4}
@@ -66,13 +66,20 @@ class RotaryTable:
         # turns a position, in units of 2^-64 (the bits of an unsigned number)
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns],
                                   dtype=torch.int64, device=device)
+        self.turns_ptr, self.device_index = self.turns.data_ptr(), self.turns.get_device()
 
 
-def _rows(t, name: str, dev: int):
-    kind = _kind(t, name, dev, _FLOATS)
+def _rows(t, name: str, dev: int, kinds):
+    _kind(t, name, dev, kinds)
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim]")
-    return _lib.Tensor3D(t.data_ptr(), *t.shape, *t.stride()), kind
+    return _lib.Tensor3D(t.data_ptr(), *t.shape, *t.stride())
+
+
+def _new(like, d):
+    """A contiguous result of like's shape (descriptor d), and its descriptor."""
+    t = like.new_empty(like.shape)
+    return t, _lib.Tensor3D(t.data_ptr(), d.dim0, d.dim1, d.dim2, d.dim1 * d.dim2, d.dim2, 1)
 
 
 def rotary(q, k, positions, table: RotaryTable, *, interleaved: bool = False,
@@ -92,35 +99,35 @@ def rotary(q, k, positions, table: RotaryTable, *, interleaved: bool = False,
         _FLOATS = {torch.bfloat16: LLK_BF16, torch.float32: LLK_FP32}
         _INT32 = {torch.int32: 0}
     dev = _begin()
-    qd, kind = _rows(q, "q", dev)
+    qd = _rows(q, "q", dev, _FLOATS)
+    kind = _FLOATS[q.dtype]
     kd = kod = None
     if k is not None:
-        kd, other = _rows(k, "k", dev)
-        if other != kind:
+        kd = _rows(k, "k", dev, _FLOATS)
+        if k.dtype is not q.dtype:
             raise ValueError("q and k have different types")
+    elif k_out is not None:
+        raise ValueError("k_out without k")
     _kind(positions, "positions", dev, _INT32)
     if positions.dim() != 1 or positions.shape[0] != qd.dim0:
         raise ValueError("positions must be [tokens]")
     if qd.dim0 > 1 and positions.stride(0) != 1:
         raise ValueError("positions must be contiguous")
-    if table.turns.get_device() != dev:
+    if table.device_index != dev:
         raise ValueError("table is not on the current device")
-
-    def result(given, like, name):
-        if given is None:
-            given = _result(like, like.dtype)
-        d, other = _rows(given, name, dev)
-        if other != kind:
-            raise ValueError(f"{name} must have q's type")
-        return given, d
-
-    q_out, qod = result(q_out, q, "q_out")
+    if q_out is None:
+        q_out, qod = _new(q, qd)
+    else:
+        qod = _rows(q_out, "q_out", dev, _FLOATS)
     if k is not None:
-        k_out, kod = result(k_out, k, "k_out")
-    elif k_out is not None:
-        raise ValueError("k_out without k")
-    check(lib().llk_rotary(qd, kd, positions.data_ptr(), table.turns.data_ptr(),
-                           table.rotary_dim // 2, table.attention_factor, kind,
+        if k_out is None:
+            k_out, kod = _new(k, kd)
+        else:
+            kod = _rows(k_out, "k_out", dev, _FLOATS)
+    if q_out.dtype is not q.dtype or (k is not None and k_out.dtype is not q.dtype):
+        raise ValueError("q_out and k_out must have q's type")
+    check(lib().llk_rotary(qd, kd, positions.data_ptr(), table.turns_ptr, table.rotary_dim // 2,
+                           table.attention_factor, kind,
                            (1 if interleaved else 0) | (2 if inverse else 0), qod, kod,
                            _context(dev, stream)))
     return q_out, k_out

@@ -38,6 +38,15 @@ def _matrix(t, name: str, dev: int, kinds):
     return _rows(t, name), kind
 
 
+def _result(x, m: int, n: int, dtype, kinds):
+    """An uninitialised [m, n] result beside x, its descriptor and its kind."""
+    kind = kinds.get(dtype)
+    if kind is None:
+        raise ValueError(f"out_dtype {dtype} unsupported; expected one of {tuple(kinds)}")
+    out = x.new_empty((m, n), dtype=dtype)
+    return out, _lib.Tensor2D(out.data_ptr(), m, n, n, 1), kind
+
+
 def q4_quantise(w, *, group: int = 128, zeros: bool = False, scale_dtype=None, stream=None):
     """(codes uint8 [K, N], scales [groups, N], zeros uint8 [groups, N] or None)
     of bf16 weights [K, N] on the current device.
@@ -117,8 +126,9 @@ def q4_matmul(x, w: Q4Weights, *, out=None, out_dtype=None, accumulate: bool = F
     if out is None:
         if accumulate:
             raise ValueError("accumulate=True needs `out`, the accumulator")
-        out = x.new_empty((xd.dim0, w.N), dtype=out_dtype or _torch().float32)
-    od, kind = _matrix(out, "out", dev, _OUT)
+        out, od, kind = _result(x, xd.dim0, w.N, out_dtype or _torch().float32, _OUT)
+    else:
+        od, kind = _matrix(out, "out", dev, _OUT)
     check(lib().llk_q4_gemm(xd, wc, od, kind, accumulate,
                             _context(dev, stream, scratch)))
     return out
@@ -132,8 +142,9 @@ def q4_swiglu(x, wg: Q4Weights, wu: Q4Weights, *, out=None, out_dtype=None, stre
     gc, uc = _packed(wg, "wg", dev), _packed(wu, "wu", dev)
     xd, _ = _matrix(x, "x", dev, _BF16)
     if out is None:
-        out = x.new_empty((xd.dim0, wg.N), dtype=out_dtype or _torch().bfloat16)
-    od, kind = _matrix(out, "out", dev, _SUMS)
+        out, od, kind = _result(x, xd.dim0, wg.N, out_dtype or _torch().bfloat16, _SUMS)
+    else:
+        od, kind = _matrix(out, "out", dev, _SUMS)
     check(lib().llk_q4_swiglu(xd, gc, uc, od, kind, _context(dev, stream, scratch)))
     return out
 
