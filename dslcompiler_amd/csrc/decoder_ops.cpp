@@ -485,8 +485,10 @@ int llk_kv4_write_marked(const llk_tensor3d* k, const llk_tensor3d* v, const llk
   Kv4Rows r;
   Kv4Marks m;
   bool empty = false;
-  int rc = check_move(k, v, cache, batch, false, &c, &b, &r, &empty);
-  if (rc || (rc = check_marks(marks, cache->pages, cache->heads, cache->page_size, 0, &m))) return rc;
+  int rc = check_cache(cache, &c);
+  if (rc || (rc = check_marks(marks, cache->pages, cache->heads, cache->page_size, 0, &m)) ||
+      (rc = check_move(k, v, cache, batch, false, &c, &b, &r, &empty)))
+    return rc;
   if (empty) return LLK_OK;
   const hipError_t e =
       llk_launch_kv4_write(c, b, r, (int)cache->head_dim, stream_of(ctx), &m, at);
@@ -531,8 +533,8 @@ int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads,
   if (params->keep < 1 || params->keep > kKv4MaxLength)
     return fail(LLK_ERR_SHAPE, "keep %lld unsupported (1 to %d)", (long long)params->keep,
                 kKv4MaxLength);
-  if (params->recent < 0 || params->first < 0 || params->recent + params->first > params->keep ||
-      params->recent > params->keep || params->first > params->keep)
+  if (params->recent < 0 || params->first < 0 || params->recent > params->keep ||
+      params->first > params->keep - params->recent)
     return fail(LLK_ERR_INVALID_ARGUMENT, "recent %lld and first %lld are negative or beyond keep %lld",
                 (long long)params->recent, (long long)params->first, (long long)params->keep);
   const bool guarded = params->recent > 0 || params->first > 0;
@@ -568,18 +570,17 @@ int llk_kv4_evict(const llk_kv4_cache* cache, const llk_kv4_batch* batch, const 
   int rc;
   if ((rc = check_cache(cache, &c))) return rc;
   if (!batch) return fail(LLK_ERR_INVALID_ARGUMENT, "batch is NULL");
+  if (batch->sequences > 0 && !source) return fail(LLK_ERR_INVALID_ARGUMENT, "source is NULL");
   llk_kv4_batch used = *batch;  // its table and sequences
-  used.lens = used.table;
+  used.lens = source;           // (not read)
   used.starts = nullptr;
   used.tokens = used.sequences;
-  if (used.table_pages == 0) used.sequences = used.tokens = 0;  // no slots
   if ((rc = check_batch(&used, &b))) return rc;
   if (keep < 1 || keep > kKv4MaxLength)
     return fail(LLK_ERR_SHAPE, "keep %lld unsupported (1 to %d)", (long long)keep, kKv4MaxLength);
   if (marks && (rc = check_marks(marks, cache->pages, cache->heads, cache->page_size, 0, &m))) return rc;
   if ((rc = check_heads(b, cache->heads))) return rc;
   if (b.sequences == 0) return LLK_OK;
-  if (!source) return fail(LLK_ERR_INVALID_ARGUMENT, "source is NULL");
   int dev;
   if ((rc = llk::current_gfx950(&dev))) return rc;
   const hipError_t e = llk_launch_kv4_evict(c, b, m, source, (int)keep, lens, (int)cache->head_dim,

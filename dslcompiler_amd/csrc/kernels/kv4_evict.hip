@@ -425,6 +425,9 @@ hipError_t llk_launch_kv4_evict_plan(const Kv4EvictPlan& p, int64_t max_len, hip
   using namespace llk_gfx950;
   int64_t len = (int64_t)p.batch.table_pages << p.page_shift;
   if (max_len > 0) len = std::min(len, max_len);
+  // Slots in registers: 2, 8 or 16 to a thread; a longer sequence reads its marks at
+  // every pass.  Measured, us, of 64 sequences of 8 heads: 2000 slots 12.5, 27.3 and
+  // 53.7; 8000 slots 117 (at every pass), 20.1 and 47.6.
   return len <= 2048 ? plan<2, 1024>(p, s) : len <= 8192 ? plan<8, 1024>(p, s) : plan<16, 1024>(p, s);
 }
 

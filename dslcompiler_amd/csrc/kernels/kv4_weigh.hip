@@ -403,7 +403,7 @@ hipError_t llk_launch_kv4_weigh(const Kv4AttentionArgs& args, const Kv4Marks& m,
   }
   const int64_t all = (len + kStep - 1) / kStep;  // steps of a sequence, at most
   // about 8192 waves; with kept scores 256 keys to a wave
-  int steps = a.kept ? 8 : (int)std::max<int64_t>(1, all * groups / 8192);
+  int steps = a.kept ? 8 : (int)std::clamp<int64_t>(all * groups / 8192, 1, all);
   void* params[] = {&a, &marks, &decay, &steps};
   const void* fn =
       a.kept ? (D == 64    ? reinterpret_cast<const void*>(&kv4_weigh_kernel<64, true>)

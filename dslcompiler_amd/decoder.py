@@ -340,7 +340,8 @@ def kv4_evict_plan(weights, table, lens, keep: int, *, positions=None, recent: i
         _kind(lens_out, "lens_out", dev, _INT32)
         if lens_out.shape != lens.shape or (lens.shape[0] > 1 and lens_out.stride(0) != 1):
             raise ValueError("lens_out must be a contiguous vector like lens")
-    source = lens.new_empty((batch.sequences, heads, max(keep, 0)))
+    # (a keep that the call refuses takes no memory)
+    source = lens.new_empty((batch.sequences, heads, keep if 0 < keep <= 1 << 30 else 0))
     check(lib().llk_kv4_evict_plan(marks, pages, heads, size, batch,
                                    _lib.EvictParams(keep, recent, first), lens_out.data_ptr(),
                                    source.data_ptr(), _context(dev, stream)))

@@ -258,3 +258,24 @@ def test_refusals(llk, gpu):
     cache = gpu.zeros(w.shape[0], 2, 17 * 64, dtype=gpu.uint8, device="cuda")
     with pytest.raises(ValueError, match="source"):
         llk.kv4_evict(cache, table, gpu.zeros(1, 3, 4, dtype=gpu.int32, device="cuda"), head_dim=64)
+
+
+@pytest.mark.parametrize("hint", [1, 100, 2048, 3000, 9000])
+def test_a_hint_below_the_lengths(llk, gpu, hint):
+    """Any max_len gives the same plan."""
+    pool = Pool(gpu, [2000, 5000, 2049, 8193, 100], 2, 64, hint, ties=hint > 1000)
+    for keep in (60, 2000, 4000):
+        pool.check(llk, keep, recent=20, first=4, max_len=hint)
+        pool.check(llk, keep, with_positions=False, max_len=hint)
+
+
+def test_lengths_are_cut_without_pages(llk, gpu):
+    cache = gpu.zeros(3, 2, 17 * 64, dtype=gpu.uint8, device="cuda")
+    table, source = gpu.zeros(2, 0, dtype=gpu.int32, device="cuda"), \
+        gpu.zeros(2, 2, 5, dtype=gpu.int32, device="cuda")
+    lens = gpu.tensor([9, 3], dtype=gpu.int32, device="cuda")
+    new, plan_source = llk.kv4_evict_plan(gpu.zeros(3, 2, 16, device="cuda"), table, lens, 5)
+    assert new.tolist() == [5, 3]
+    assert gpu.equal(plan_source, gpu.arange(5, device="cuda").int().expand(2, 2, 5))
+    llk.kv4_evict(cache, table, source, head_dim=64, lens=lens)
+    assert lens.tolist() == [5, 3] and (cache == 0).all()

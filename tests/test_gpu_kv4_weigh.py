@@ -226,3 +226,60 @@ def test_written_marks(llk, gpu, heads, page):
     assert np.array_equal(p.cpu().numpy(), wp)
     with pytest.raises(ValueError, match="at"):
         llk.kv4_write(kv, kv, pool, table, lens_d, starts=starts, at=at)
+
+
+@pytest.mark.parametrize("news,group", [([1, 1, 1], 4), ([1, 1, 1], 20), ([3, 2, 1], 2), ([140, 200, 129], 2)])
+def test_a_hint_below_the_lengths(llk, gpu, news, group):
+    """Any max_len gives right sums: scores are kept of the first keys only, or fewer
+    workgroups go round."""
+    lens = [n + extra for n, extra in zip(news, (700, 30, 1500))]
+    c = Case(gpu, lens, news, 2, 64, 32, seed=group)
+    q = c.queries(2 * group)
+    for hint in (1, 256, 300, 1024):
+        run(llk, c, q, 0.5, max_len=hint)
+        run(llk, c, q, 1.0, max_len=hint, window=400, sinks=10)
+
+
+def test_single_tokens_given_by_starts(llk, gpu):
+    """With `starts` no scores are kept; the sums are the same."""
+    c = Case(gpu, [300, 41, 513], [1, 1, 1], 2, 128, 16, seed=2)
+    pool, table, lens, _ = c.dev()
+    q = _dev(gpu, c.queries(8), gpu.bfloat16)
+    got = []
+    for starts in (None, gpu.arange(4, device="cuda").int()):
+        w = gpu.zeros(pool.shape[0], 2, 16, device="cuda")
+        llk.kv4_attention(q, pool, table, lens, starts=starts, weights=w)
+        got.append(w)
+    # each within this file's bound, its keys being below 6
+    near = 144 * 2.0 ** -22 * 128 ** -0.5 * 6 * float(q.float().abs().sum(-1).max()) + 2.0 ** -18
+    assert ((got[0] - got[1]).abs() <= 2 * near * gpu.maximum(*got)).all()
+    rows = gpu.stack(got).double().sum((1, 3))
+    assert ((rows - 3 * 4).abs() <= 12 * near).all()  # 3 tokens, 4 query heads, a sum of 1 each
+
+
+def test_weights_beyond_32_bits(llk, gpu):
+    """Pages of the cache and of the marks at offsets beyond 2^32 bytes."""
+    D, size = 64, 16
+    c = Case(gpu, [40, 20], [1, 1], 2, D, size, seed=4)
+    q = _dev(gpu, c.queries(4), gpu.bfloat16)
+    pool, table, lens, _ = c.dev()
+    pages = pool.shape[0]
+    step = ((1 << 32) + 4096) // (pages - 1) // 16 * 16 + 16
+    far = gpu.empty(pages * step, dtype=gpu.uint8, device="cuda").as_strided(
+        pool.shape, (step, pool.shape[2], 1))
+    far.copy_(pool)
+    marks = gpu.empty(pages * step // 4, dtype=gpu.float32, device="cuda").as_strided(
+        (pages, 2, size), (step // 4, size, 1))
+    marks.fill_(1.0)
+    near = gpu.ones(pages, 2, size, device="cuda")
+    a = llk.kv4_attention(q, pool, table, lens, weights=near)
+    b = llk.kv4_attention(q, far, table, lens, weights=marks)
+    assert gpu.equal(a, b) and gpu.equal(near, marks)
+    k = gpu.randn(2, 2, D, device="cuda").bfloat16()
+    llk.kv4_write(k, k, pool, table, lens, weights=near)
+    llk.kv4_write(k, k, far, table, lens, weights=marks)
+    assert gpu.equal(pool, far) and gpu.equal(near, marks)
+    for x, w in ((pool, near), (far, marks)):
+        _, source = llk.kv4_evict_plan(w, table, lens, 17)
+        llk.kv4_evict(x, table, source, head_dim=D, weights=w)
+    assert gpu.equal(pool, far) and gpu.equal(near, marks)
