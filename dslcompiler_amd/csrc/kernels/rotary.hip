@@ -6,7 +6,8 @@
 // signed number, give the angle to 2^-32 of a turn, and fp32 keeps 24 bits of it.
 //
 // HBM bound.  The cosines and sines of a workgroup's tokens are computed once,
-// into LDS, and serve all heads of q and k.
+// into LDS, and serve all heads of q and k.  16384 tokens of 32 + 8 heads of 128, bf16:
+// 57.8 us, 5.8 TB/s of reads and writes (partly from the last-level cache).
 #include <algorithm>
 
 #include "common.h"
@@ -144,11 +145,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a, int per) {
 template <bool F32, bool SIDE_BY_SIDE>
 hipError_t launch(const RotaryArgs& args, hipStream_t s) {
   RotaryArgs a = args;
-  // 256 cosines to a workgroup, and LDS for at most so many; few tokens: one to
-  // a workgroup
-  int per = std::max(1, std::min(256 / a.pairs, a.tokens / 512));
-  void* params[] = {&a, &per};
   const bool wide = a.pairs % 8 == 0;
+  const int items = (a.side[0].heads + a.side[1].heads) * (wide ? a.pairs / 8 : a.pairs);
+  // An item to a thread, not more than 256 cosines, and two workgroups to a CU.
+  // Measured, us, 1, 2, 4 and 8 tokens to a workgroup: 16384 tokens, 40 heads of 128,
+  // 57.8, 59.0, 60.9, 60.6; 9 heads of 64 15.8, 10.4, 8.5, 7.5; 64 tokens, 40 heads of
+  // 128, 3.0, 3.4, 4.1.
+  int per = std::max(1, std::min(std::min(256 / a.pairs, 256 / items), a.tokens / 512));
+  void* params[] = {&a, &per};
   return hipLaunchKernel(wide ? reinterpret_cast<const void*>(&rotary_kernel<F32, SIDE_BY_SIDE, true>)
                               : reinterpret_cast<const void*>(&rotary_kernel<F32, SIDE_BY_SIDE, false>),
                          dim3((a.tokens + per - 1) / per), dim3(256), params,
