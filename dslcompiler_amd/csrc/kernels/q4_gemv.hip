@@ -199,7 +199,7 @@ hipError_t launch_group(const Q4Args& a, const Q4Plan& p, hipStream_t s) {
 Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
   const int64_t units = std::max<int64_t>(1, q4_units(K));
   Q4Plan p{};
-  int64_t s;  // splits of K  // splits
+  int64_t s;  // splits of K
   const int64_t columns = q4_tiles(N);
   if (M <= 16 || K < 8) {  // (the tile kernel reads 8 elements of a row at once)
     // A workgroup's X takes 256 M bytes a unit of K.  Without a split of K a call is one
@@ -223,9 +223,13 @@ Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
       s = std::max((x + 319) / 320, std::min(480 / four, units / 8));
     }
   } else {
-    p.rows = M <= 32 ? 32 : 64;
+    // 64 rows read the codes half as often, 32 leave more workgroups that hide their
+    // waits.  Measured, us, 32 and 64: 4096 x 4096, 64 rows, 15.3, 18.7, 128 rows 21.8,
+    // 23.6; 13824 x 5120, 255 rows, 75.6, 68.6; SwiGLU of 4096 x 14336, 64 rows, 35.5, 35.1.
+    p.rows = M <= 128 ? 32 : 64;
     const int64_t tiles = (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256);
-    // two workgroups to a CU, at least 4 units to each
+    // Two workgroups to a CU, at least 4 units to each.  SwiGLU of 4096 x 14336, 32 rows:
+    // 512 workgroups 23.5 us, 768 26.3, 1024 28.0; 13824 x 5120, 17 rows, 18.8, 20.6, 20.6.
     s = std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, units / 4));
   }
   p.stages = (int)((units + s - 1) / s);

@@ -248,3 +248,66 @@ def test_streams_and_graph(llk, gpu):
             x.copy_(gpu.randn(*x.shape, device="cuda"))
             graph.replay()
             assert gpu.equal(out, llk.q4_matmul(x, w)) and gpu.equal(both, llk.q4_swiglu(x, w, w))
+
+
+@pytest.mark.parametrize("M,K,N", [(17, 1, 16), (20, 5, 33), (100, 7, 16), (1000, 3, 40), (17, 8, 16),
+                                   (129, 9, 300)])
+def test_many_rows_of_few_values(llk, gpu, M, K, N):
+    for group in (32, 128):
+        x, codes, scales, z = case(gpu, M, K, N, group, True, gpu.bfloat16, M + K, True)
+        w = llk.Q4Weights.from_codes(codes, scales, z, group=group)
+        want = f64(x) @ dense(codes, scales, z, group)
+        assert np.array_equal(f64(llk.q4_matmul(x, w)), want)
+        both = llk.q4_swiglu(x, w, w, out_dtype=gpu.float32)
+        # exact sums: only the activation's 4 ulp, of its exponent's argument two
+        # roundings of |sum| 2^-24, and its product
+        with np.errstate(over="ignore"):
+            silu = want / (1 + np.exp(-want))
+        near = (np.abs(want) + 8) * 2.0 ** -23 * np.abs(silu * want) + 1e-30
+        assert (np.abs(f64(both) - silu * want) <= near).all()
+
+
+@pytest.mark.parametrize("M", [1, 12, 30, 200])
+def test_sums_added_to_half_precision(llk, gpu, M):
+    """One rounding of what is there plus the product (exact cases, so equal)."""
+    K, N, group = 500, 48, 32
+    x, codes, scales, z = case(gpu, M, K, N, group, False, gpu.bfloat16, M, True)
+    w = llk.Q4Weights.from_codes(codes, scales, z, group=group)
+    want = f64(x) @ dense(codes, scales, z, group)
+    for t in (gpu.float16, gpu.bfloat16):
+        acc = gpu.randint(-64, 64, (M, N), device="cuda").to(t)
+        total = gpu.from_numpy(want + f64(acc)).float().cuda().to(t)
+        assert gpu.equal(llk.q4_matmul(x, w, out=acc, accumulate=True), total)
+
+
+@pytest.mark.parametrize("M,K,N,sides", [(5, 13824, 256, 1), (40, 4096, 512, 2), (300, 5000, 80, 1)])
+def test_a_workspace_of_the_callers(llk, gpu, M, K, N, sides):
+    """Split products in memory of the caller's, exactly as large as is asked for,
+    with its neighbours untouched; one that is too small is refused."""
+    x, codes, scales, z = case(gpu, M, K, N, 128, True, gpu.bfloat16, 1, False)
+    w = llk.Q4Weights.from_codes(codes, scales, z, group=128)
+
+    def call(**kw):
+        return llk.q4_matmul(x, w, **kw) if sides == 1 else llk.q4_swiglu(x, w, w, **kw)
+
+    need = llk.q4_scratch_size(M, N, K, sides)
+    assert need > 0
+    memory = gpu.full((need + 512,), 7, dtype=gpu.uint8, device="cuda")
+    assert gpu.equal(call(scratch=memory[256:256 + need]), call())
+    assert (memory[:256] == 7).all() and (memory[256 + need:] == 7).all()
+    with pytest.raises(llk.LLKError):
+        call(scratch=memory[256:need])
+
+
+def test_rows_far_apart(llk, gpu):
+    """Offsets of X and Y beyond 2^32 bytes."""
+    K, N = 64, 32
+    for M in (16, 40):
+        step = (1 << 31) // (M - 4)
+        x, codes, scales, z = case(gpu, M, K, N, 64, True, gpu.bfloat16, M, True)
+        w = llk.Q4Weights.from_codes(codes, scales, z, group=64)
+        far = gpu.empty(M * step, dtype=gpu.bfloat16, device="cuda").as_strided((M, K), (step, 1))
+        far.copy_(x)
+        out = gpu.empty(M * step, dtype=gpu.float32, device="cuda").as_strided((M, N), (step, 1))
+        llk.q4_matmul(far, w, out=out)
+        assert np.array_equal(f64(out), f64(x) @ dense(codes, scales, z, 64))
