@@ -84,12 +84,18 @@ namespace llk_gfx950 {
 
 constexpr uint32_t kCodeMask = 0x00780078u, kCodeOne = 0x3f803f80u;
 
+// kCodeOne in a vector register, which the compiler would not keep there by itself: with
+// it v_and_or_b32 takes both constants, one of them a scalar.
+__device__ __forceinline__ uint32_t q4_one() {
+  uint32_t one;
+  asm("v_mov_b32 %0, %1" : "=v"(one) : "s"(kCodeOne));
+  return one;
+}
 // A dword's 8 codes as bf16 1 + c / 16.
-__device__ __forceinline__ bf16x8 q4_decode8(uint32_t q) {
+__device__ __forceinline__ bf16x8 q4_decode8(uint32_t q, uint32_t one) {
   return __builtin_bit_cast(
-      bf16x8, u32x4{(q & kCodeMask) | kCodeOne, ((q >> 4) & kCodeMask) | kCodeOne,
-                    ((q >> 8) & kCodeMask) | kCodeOne,
-                    (__builtin_amdgcn_alignbit(q, q, 12) & kCodeMask) | kCodeOne});
+      bf16x8, u32x4{(q & kCodeMask) | one, ((q >> 4) & kCodeMask) | one, ((q >> 8) & kCodeMask) | one,
+                    (__builtin_amdgcn_alignbit(q, q, 12) & kCodeMask) | one});
 }
 __device__ __forceinline__ float q4_scale(uint32_t w) { return __uint_as_float(w & 0xffffe000u); }
 // -(1 + z / 16)

@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_gemv_kernel(Q4Args a) {
 #pragma unroll
     for (int i = 0; i < MR; ++i) acc[s][i] = 0.0f;
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{kCodeOne, kCodeOne, kCodeOne, kCodeOne});
+  const uint32_t code_one = q4_one();
   auto work = [&](int u, const Unit& o) {
     constexpr int kSteps = 4 / kGroups;  // of 32 k, to a group
     const u32x4* const xs = lds + ((u - begin) * rows + row) * 16;
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_gemv_kernel(Q4Args a) {
         sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, ones, sx, 0, 0, 0);
 #pragma unroll
         for (int s = 0; s < SIDES; ++s)
-          part[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, q4_decode8(o.codes[s][j]), part[s], 0, 0, 0);
+          part[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, q4_decode8(o.codes[s][j], code_one), part[s], 0, 0, 0);
       }
 #pragma unroll
       for (int s = 0; s < SIDES; ++s) {

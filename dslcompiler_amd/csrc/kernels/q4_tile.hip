@@ -125,7 +125,16 @@ __global__ void __launch_bounds__(kWaves * 64)
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int c = 0; c < kTiles; ++c) acc[r][c] = f32x4{0, 0, 0, 0};
+  const uint32_t code_one = q4_one();
   auto work = [&](int buf, const Codes& w) {
+    bf16x8 x[2][RT];  // operands of a step, the next one's on their way
+    auto read = [&](int j) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        x[j & 1][r] =
+            __builtin_bit_cast(bf16x8, xs[buf][(j * RT + r) * 64 + grp * 16 + (col ^ (4 * j + grp))]);
+    };
+    read(0);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       f32x4 part[RT][kTiles];
@@ -135,16 +144,14 @@ __global__ void __launch_bounds__(kWaves * 64)
         for (int c = 0; c < kTiles; ++c) part[r][c] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int j = g * kSteps; j < (g + 1) * kSteps; ++j) {
-        bf16x8 x[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-          x[r] = __builtin_bit_cast(bf16x8, xs[buf][(j * RT + r) * 64 + grp * 16 + (col ^ (4 * j + grp))]);
+        if (j < 3) read(j + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
-          const bf16x8 q = q4_decode8(w.q[c][j]);
+          const bf16x8 q = q4_decode8(w.q[c][j], code_one);
 #pragma unroll
           for (int r = 0; r < RT; ++r)
-            part[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[r], q, part[r][c], 0, 0, 0);
+            part[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[j & 1][r], q, part[r][c], 0, 0, 0);
         }
       }
       f32x4 sx[RT];
