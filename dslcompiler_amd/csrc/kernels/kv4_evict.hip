@@ -9,8 +9,13 @@
 // that stay.  So few bytes move however long the cache is, and none is read after it
 // was written: sources lie from `keep` on, targets below.
 //
+// What bounds it is the chain of its passes: one sequence's 8 heads 10 us, 512 heads of
+// up to 8192 slots 28 us (36 with two bits of the key a pass, counted by ballots).
+//
 // Move: a lane to a slot below `keep`, with all of its token's blocks on their way at
-// once.
+// once.  HBM: a token's 16 bytes of every 256 and its scales' single bytes are parts of
+// lines that are moved whole.  512 heads 64 us; with loads that stay in the caches 90,
+// with the blocks of a token on neighbouring lanes 101.
 #include <algorithm>
 
 #include "common.h"

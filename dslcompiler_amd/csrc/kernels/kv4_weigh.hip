@@ -10,7 +10,9 @@
 // Single tokens (few rows): the attention stores its scores, 4 bytes for a row and key
 // where the cache has 17/16 D, and they are read once more here.  Where it did not,
 // or rows are many, the scores are computed again: a prompt has far more pairs of a
-// row and a key than could be kept.
+// row and a key than could be kept.  64 ragged sequences to 8192 keys, 32 query heads
+// on 8: the attention 84 us with its scores stored (68 without) and 15 here, a call
+// 108 in all, and 156 with the scores computed again.
 #include <algorithm>
 #include <type_traits>
 

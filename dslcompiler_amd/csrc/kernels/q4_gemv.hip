@@ -16,7 +16,9 @@
 // to LDS once (read as operands from memory they are four times a unit's codes, and
 // the vector memory path, not HBM, would be the limit), and its 8 waves take the
 // range's units in turn, four of them on their way.  Their sums are joined in LDS, and
-// those of a split K by a second kernel.
+// those of a split K by a second kernel.  SwiGLU of 4096 x 14336, 1 row: 12.3 us, 5.0
+// TB/s; 13824 x 5120, 5 rows: 11.4 us and 4.0 to join 6 splits.  With X from memory
+// 15.8 and 18.7.
 #include <algorithm>
 
 #include "common.h"

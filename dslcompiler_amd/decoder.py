@@ -298,7 +298,8 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
 
     weights (of :func:`kv4_marks`): in every slot of a sequence with new tokens,
     decay times what was there (with 0 it is not read) plus the softmax weights
-    that the new tokens' query heads gave it."""
+    that the new tokens' query heads gave it.  A page that is in the table twice
+    (a prefix that two sequences share) gets sums without order."""
     dev = _begin()
     args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev)
     if out is None:
@@ -352,7 +353,8 @@ def kv4_evict(cache, table, source, *, head_dim: int, weights=None, positions=No
               stream=None) -> None:
     """Moves the cache's tokens, and their marks if given, as `source` of
     :func:`kv4_evict_plan` says; lens, if given, is cut to source's `keep` in
-    place.  The pages behind the new lengths are free."""
+    place.  The pages behind the new lengths are free.  A page that two sequences
+    share would be changed for both: copy it before."""
     dev = _begin()
     cd = _cache(cache, head_dim, dev)
     marks = _marks(weights, positions, (cd.pages, cd.heads, cd.page_size), dev)

@@ -311,8 +311,8 @@ int llk_block_norm(const llk_tensor2d* y, const llk_tensor2d* residual,
                    llk_tensor2d* residual_out, llk_tensor2d* out,
                    const llk_block_norm_params* params, llk_kernel_context* ctx);
 
-/* [dim0, dim1, dim2] (bf16 where nothing else is said) with unit stride2; stride0 and stride1 in elements,
- * in either order (rows of a result must not overlap). */
+/* [dim0, dim1, dim2] (bf16 where nothing else is said) with unit stride2; stride0
+ * and stride1 in elements, in either order (rows of a result must not overlap). */
 typedef struct llk_tensor3d {
   void* data;
   int64_t dim0, dim1, dim2;
@@ -431,7 +431,8 @@ int llk_kv4_write_marked(const llk_tensor3d* k, const llk_tensor3d* v, const llk
  * sequence with new tokens, each of its first lens[s] slots and each head,
  *   marks.weights = decay * marks.weights + sum of the softmax weights that the new
  *   tokens' query heads of that head gave the slot (0 from those that do not see it);
- * with decay 0 what was there is not read.  In fp32, and the same from run to run.
+ * with decay 0 what was there is not read.  In fp32, and the same from run to run if
+ * no page is in the tables twice (two sequences that share one add up without order).
  * Other slots are left as they are.  A row without a key it sees adds nothing, one
  * that is NaN makes the slots that it sees NaN.  The result is that of
  * llk_kv4_attention, bit for bit. */
@@ -457,8 +458,8 @@ typedef struct llk_kv4_evict_params {
  * the others below keep, in order, take those from keep on that stay, in order:
  * source[s][head][i], int32 [sequences][heads][keep], is the slot that slot i takes
  * its token from, i itself if it does not change.  lens: the new lengths, the
- * smaller of batch.lens and keep (not batch.lens itself, which every head reads).  Of batch, table,
- * lens and sequences are read.  Nothing is moved. */
+ * smaller of batch.lens and keep (not batch.lens itself, which every head reads).
+ * Of batch, table, lens and sequences are read.  Nothing is moved. */
 int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads, int64_t page_size,
                        const llk_kv4_batch* batch, const llk_kv4_evict_params* params,
                        int32_t* lens, int32_t* source, llk_kernel_context* ctx);
@@ -466,8 +467,9 @@ int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads,
 /* Moves tokens to the slots below `keep` as `source` (of llk_kv4_evict_plan) says,
  * keys and values and, unless NULL, marks.  Slots are moved only from keep on, and
  * only where both pages exist.  lens, unless NULL: lengths on the device that are
- * cut to keep.  The pages behind the new lengths are the caller's again.  Of batch,
- * table and sequences are read. */
+ * cut to keep.  The pages behind the new lengths are the caller's again.  A page must
+ * be in the tables once: one that two sequences share is changed for both.  Of
+ * batch, table and sequences are read. */
 int llk_kv4_evict(const llk_kv4_cache* cache, const llk_kv4_batch* batch, const int32_t* source,
                   int64_t keep, const llk_kv4_marks* marks, int32_t* lens, llk_kernel_context* ctx);
 
