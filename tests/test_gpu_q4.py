@@ -311,3 +311,26 @@ def test_rows_far_apart(llk, gpu):
         out = gpu.empty(M * step, dtype=gpu.float32, device="cuda").as_strided((M, N), (step, 1))
         llk.q4_matmul(far, w, out=out)
         assert np.array_equal(f64(out), f64(x) @ dense(codes, scales, z, 64))
+
+
+@pytest.mark.parametrize("M,K,N,sides", [(15, 5000, 13824, 1), (14, 5120, 12800, 2)])
+def test_a_first_call_under_capture(llk, gpu, M, K, N, sides):
+    """A launch with more than 64 KiB of LDS that nothing made before the capture."""
+    x, codes, scales, z = case(gpu, M, K, N, 64, True, gpu.float16, 8, False)
+    w = llk.Q4Weights.from_codes(codes, scales, z, group=64)
+    scratch = gpu.empty(max(llk.q4_scratch_size(M, N, K, sides), 256), dtype=gpu.uint8, device="cuda")
+
+    def call():
+        return llk.q4_matmul(x, w, scratch=scratch) if sides == 1 else \
+            llk.q4_swiglu(x, w, w, scratch=scratch)
+
+    side = gpu.cuda.Stream()
+    gpu.cuda.synchronize()
+    graph = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(graph, stream=side):
+        out = call()
+    for _ in range(3):
+        x.copy_(gpu.randn(*x.shape, device="cuda"))
+        graph.replay()
+        gpu.cuda.synchronize()
+        assert gpu.equal(out, call())
