@@ -202,6 +202,7 @@ hipError_t launch_group(const Q4Args& a, const Q4Plan& p, hipStream_t s) {
 Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
   const int64_t units = std::max<int64_t>(1, q4_units(K));
   Q4Plan p{};
+  if (M == 0 || N == 0) return p;  // no launch
   int64_t s;  // splits of K
   const int64_t columns = q4_tiles(N);
   if (M <= 16 || K < 8) {  // (the tile kernel reads 8 elements of a row at once)

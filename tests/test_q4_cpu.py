@@ -74,6 +74,15 @@ def test_product_refusals(L):
     assert L.llk_q4_gemm(x, _w(N=0), _t(4, 0), 0, 0, None) == 0
 
 
+@pytest.mark.parametrize("sides", [1, 2])
+@pytest.mark.parametrize("M,N,K", [(16, 0, 4096), (1, 0, 65535 * 32), (3, 0, 65535 * 32), (17, 0, 4096),
+                                   (0, 4096, 4096), (0, 0, 4096), (16, 0, 0), (0, 0, 0)])
+def test_workspace_of_an_empty_product(L, M, N, K, sides):
+    """Also where X alone would not fit a workgroup, so that K would be split by
+    the number of columns."""
+    assert L.llk_q4_scratch_size(M, N, K, sides) == 0
+
+
 def test_pack_and_quantise_refusals(L):
     codes, scales = _t(256, 64), _t(4, 64)
     for bad, code in BAD_WEIGHTS:
