@@ -103,8 +103,14 @@ class Q4Weights:
     def quantise(cls, w, *, group: int = 128, zeros: bool = False, scale_dtype=None,
                  stream=None) -> "Q4Weights":
         """:func:`q4_quantise` of bf16 weights [K, N], packed."""
-        return cls.from_codes(*q4_quantise(w, group=group, zeros=zeros, scale_dtype=scale_dtype,
-                                           stream=stream), group=group, stream=stream)
+        parts = q4_quantise(w, group=group, zeros=zeros, scale_dtype=scale_dtype, stream=stream)
+        if stream is not None:
+            # dropped as this returns, when the stream may not have packed them yet: until
+            # then their memory is not to be given to the current stream's next allocations
+            for t in parts:
+                if t is not None:
+                    t.record_stream(stream)
+        return cls.from_codes(*parts, group=group, stream=stream)
 
 
 def _packed(w, name: str, dev: int) -> _lib.Q4WeightsC:

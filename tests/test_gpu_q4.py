@@ -334,3 +334,50 @@ def test_a_first_call_under_capture(llk, gpu, M, K, N, sides):
         graph.replay()
         gpu.cuda.synchronize()
         assert gpu.equal(out, call())
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_weights_made_on_a_stream_of_the_callers(llk, gpu, monkeypatch, zeros):
+    """quantise(), q4_quantise() and from_codes() on a stream that is behind: what
+    the current stream allocates and writes meanwhile is no memory of theirs."""
+    from dslcompiler_amd import q4
+    K, N, group = 1000, 1040, 64
+    w = gpu.randn(K, N, device="cuda").bfloat16()
+    want = llk.Q4Weights.quantise(w, group=group, zeros=zeros)
+    want_parts = [t for t in llk.q4_quantise(w, group=group, zeros=zeros) if t is not None]
+    parts = []
+    quantise = llk.q4_quantise
+
+    def noted(*args, **kw):
+        out = quantise(*args, **kw)
+        parts.extend((t.data_ptr(), t.numel() * t.element_size()) for t in out if t is not None)
+        return out
+
+    monkeypatch.setattr(q4, "q4_quantise", noted)
+    big = [gpu.zeros(1 << 28, dtype=gpu.uint8, device="cuda") for _ in range(2)]
+    side = gpu.cuda.Stream()
+    gpu.cuda.synchronize()
+    side.wait_stream(gpu.cuda.current_stream())
+    with gpu.cuda.stream(side):
+        for n in range(400):  # about 40 ms of copies
+            big[n % 2].copy_(big[1 - n % 2])
+    got = llk.Q4Weights.quantise(w, group=group, zeros=zeros, stream=side)
+    other = [gpu.full((size,), 0xff, dtype=gpu.uint8, device="cuda") for _, size in parts * 2]
+    if not side.query():  # it has not packed yet
+        for t in other:
+            for at, size in parts:
+                assert t.data_ptr() + t.numel() <= at or at + size <= t.data_ptr()
+    made = llk.q4_quantise(w, group=group, zeros=zeros, stream=side)
+    again = llk.Q4Weights.from_codes(*made, group=group, stream=side)
+    gpu.cuda.synchronize()
+    assert len(parts) == 2 + zeros
+    for a, b in zip([t for t in made if t is not None], want_parts):
+        assert gpu.equal(a, b)
+    x = gpu.randn(5, K, device="cuda").bfloat16()
+    first = llk.q4_matmul(x, want)
+    assert gpu.equal(llk.q4_matmul(x, got), first) and gpu.equal(llk.q4_matmul(x, again), first)
+    rows = np.arange(K) // group
+    codes, scales, z = (None if t is None else f64(t) for t in made)
+    dense64 = (codes - (8 if z is None else z[rows])) * scales[rows]
+    most = bound(x, made[1], group, K)
+    assert (np.abs(f64(first) - f64(x) @ dense64) <= most * (1 + 2.0 ** -24)).all()

@@ -119,3 +119,29 @@ def test_python_refusals(llk):
         llk.q4_matmul(w.T, w)
     with pytest.raises(ValueError, match="Q4Weights"):
         llk.q4_swiglu(w.T, w, w)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantise_keeps_its_temporaries_for_the_stream(llk, monkeypatch, zeros):
+    """The codes, scales and zeros that quantise() makes and drops are the stream's
+    until it has packed them: the allocator is told of it before it gets them back."""
+    from dslcompiler_amd import q4
+
+    class Part:
+        streams = ()
+
+        def record_stream(self, stream):
+            self.streams += (stream,)
+
+    parts = (Part(), Part(), Part() if zeros else None)
+    monkeypatch.setattr(q4, "q4_quantise", lambda w, **kw: parts)
+    monkeypatch.setattr(q4.Q4Weights, "from_codes",
+                        classmethod(lambda cls, *p, **kw: [t.streams for t in p if t is not None]))
+    stream = object()
+    seen = llk.Q4Weights.quantise(None, zeros=zeros, stream=stream)
+    assert seen == [(stream,)] * (2 + zeros)
+    for t in parts:
+        if t is not None:
+            t.streams = ()
+    # they are of the current stream's memory, which takes them in its order
+    assert llk.Q4Weights.quantise(None, zeros=zeros) == [()] * (2 + zeros)
