@@ -94,7 +94,7 @@ def rotary(q, k, positions, table: RotaryTable, *, interleaved: bool = False,
     multiplies by the same factor): the gradient of the call without it.  q_out
     and k_out may be q and k."""
     global _FLOATS, _INT32
-    if _FLOATS is None:
+    if _INT32 is None:  # the one that is set last: a second thread finds both of them, or none
         torch = _torch()
         _FLOATS = {torch.bfloat16: LLK_BF16, torch.float32: LLK_FP32}
         _INT32 = {torch.int32: 0}

@@ -23,7 +23,7 @@ _BF16 = _BYTES = _SCALES = _SUMS = _OUT = None  # torch dtype -> llk_dtype (0 fo
 def _start() -> int:
     """The current device; the tables of types on the first call."""
     global _BF16, _BYTES, _SCALES, _SUMS, _OUT
-    if _BF16 is None:
+    if _OUT is None:  # the one that is set last: a second thread finds all of them, or none
         torch = _torch()
         _BF16, _BYTES = {torch.bfloat16: LLK_BF16}, {torch.uint8: 0}
         _SCALES = {torch.bfloat16: LLK_BF16, torch.float16: LLK_FP16}
