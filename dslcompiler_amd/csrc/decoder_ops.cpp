@@ -546,9 +546,11 @@ int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads,
   if (batch->sequences == 0) return LLK_OK;
   if (!lens || !source)
     return fail(LLK_ERR_INVALID_ARGUMENT, "%s is NULL", lens ? "source" : "lens");
-  // every head's workgroup reads the old lengths
-  if (lens == batch->lens)
-    return fail(LLK_ERR_INVALID_ARGUMENT, "the new lengths must not replace batch.lens");
+  // every head's workgroup reads the old lengths, all of them while some are written
+  const uintptr_t at = reinterpret_cast<uintptr_t>(lens), old = reinterpret_cast<uintptr_t>(batch->lens);
+  const uintptr_t bytes = (uintptr_t)batch->sequences * sizeof(int32_t);
+  if (at < old + bytes && old < at + bytes)
+    return fail(LLK_ERR_INVALID_ARGUMENT, "the new lengths must not replace batch.lens, or a part of it");
   int dev;
   if ((rc = llk::current_gfx950(&dev))) return rc;
   if (!guarded) p.marks.positions = nullptr;

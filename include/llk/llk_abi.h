@@ -458,7 +458,8 @@ typedef struct llk_kv4_evict_params {
  * the others below keep, in order, take those from keep on that stay, in order:
  * source[s][head][i], int32 [sequences][heads][keep], is the slot that slot i takes
  * its token from, i itself if it does not change.  lens: the new lengths, the
- * smaller of batch.lens and keep (not batch.lens itself, which every head reads).
+ * smaller of batch.lens and keep (in memory apart from batch.lens, which every head
+ * reads).
  * Of batch, table, lens and sequences are read.  Nothing is moved. */
 int llk_kv4_evict_plan(const llk_kv4_marks* marks, int64_t pages, int64_t heads, int64_t page_size,
                        const llk_kv4_batch* batch, const llk_kv4_evict_params* params,

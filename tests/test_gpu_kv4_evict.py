@@ -279,3 +279,20 @@ def test_lengths_are_cut_without_pages(llk, gpu):
     assert gpu.equal(plan_source, gpu.arange(5, device="cuda").int().expand(2, 2, 5))
     llk.kv4_evict(cache, table, source, head_dim=64, lens=lens)
     assert lens.tolist() == [5, 3] and (cache == 0).all()
+
+
+def test_new_lengths_in_a_shifted_view(llk, gpu):
+    """Lengths and new lengths in one buffer: refused where they overlap."""
+    p = Pool(gpu, [40, 30, 20], 2, 16, 13)
+    w, pos, table, lens = p.dev()
+    both = gpu.zeros(7, dtype=gpu.int32, device="cuda")
+    old = both[2:5]
+    old.copy_(lens)
+    for at in (0, 1, 2, 3, 4):
+        with pytest.raises(llk.LLKError, match="replace"):
+            llk.kv4_evict_plan(w, table, old, 25, lens_out=both[at:at + 3])
+    assert both.tolist() == [0, 0, 40, 30, 20, 0, 0]
+    six = gpu.cat([lens, lens])
+    new, source = llk.kv4_evict_plan(w, table, six[:3], 25, lens_out=six[3:])
+    assert new.tolist() == [25, 25, 20] and six[:3].tolist() == [40, 30, 20]
+    assert gpu.equal(source, llk.kv4_evict_plan(w, table, lens, 25)[1])

@@ -137,6 +137,20 @@ def test_plan_refusals(L):
     assert call(sequences=0, tokens=0) == 0
 
 
+@pytest.mark.parametrize("sequences", [1, 2, 7])
+def test_new_lengths_apart_from_the_old_ones(L, sequences):
+    """Every head's workgroup reads batch.lens while the new lengths are written:
+    a shifted view of them is refused as they themselves are."""
+    def call(lens):
+        return L.llk_kv4_evict_plan(_marks(), 10, 2, 64, _batch(sequences=sequences, tokens=sequences),
+                                    _params(), lens, 2 * FAKE, None)
+
+    for shift in range(1 - sequences, sequences):
+        assert call(FAKE + 4 * shift) == -1 and b"replace" in L.llk_last_error(), shift
+    for shift in (-sequences, sequences):  # right beside them
+        assert call(FAKE + 4 * shift) != -1, shift
+
+
 def test_move_refusals(L):
     def call(cache=None, marks=None, keep=10, source=FAKE, lens=None, **b):
         return L.llk_kv4_evict(cache or _cache(), _batch(**b), source, keep, marks, lens, None)
