@@ -381,3 +381,69 @@ def test_weights_made_on_a_stream_of_the_callers(llk, gpu, monkeypatch, zeros):
     dense64 = (codes - (8 if z is None else z[rows])) * scales[rows]
     most = bound(x, made[1], group, K)
     assert (np.abs(f64(first) - f64(x) @ dense64) <= most * (1 + 2.0 ** -24)).all()
+
+
+def dense_on_device(torch, codes, scales, z, group):
+    """W in float64, on the device."""
+    rows = torch.arange(codes.shape[0], device="cuda") // group
+    zero = 8.0 if z is None else z.double()[rows]
+    return (codes.double() - zero) * scales.double()[rows]
+
+
+# The kernel for few rows by column tiles to a workgroup and splits of K: 1 tile below
+# 640 tiles of a product (400 of a SwiGLU), then 2, 4 for a SwiGLU from 800 on; 4 and a
+# split K where 16-row blocks of X pass 256 units (640 for a wide SwiGLU).  The sizes
+# leave no, one, two or three tiles, whole or not, to the last workgroup.
+FEW_ROWS = [(M, 300, N, sides) for M in (1, 5, 9, 16)
+            for N, sides in ((10240, 1), (10256, 1), (11000, 1), (6400, 2), (6424, 2), (12800, 2), (12840, 2))]
+FEW_ROWS += [(16, 4096, 1040, 1), (9, 5000, 1072, 1), (13, 4096, 2000, 1), (1, 33000, 100, 1),
+             (16, 4096, 11008, 2), (9, 5000, 1064, 2), (5, 8000, 1048, 2), (1, 33000, 40, 2),
+             (16, 4096, 12840, 2), (9, 5120, 12824, 2), (14, 5120, 12872, 2)]
+
+
+@pytest.mark.parametrize("M,K,N,sides", FEW_ROWS)
+def test_few_rows_of_wide_weights(llk, gpu, M, K, N, sides):
+    """Exact sums (the file's docstring; X to 1 for long K, whose sums then stay below
+    33000 * 2 < 2^17): products equal, a SwiGLU within its activation's roundings."""
+    group = (32, 64, 128)[(M + N) % 3]
+    x, *g = case(gpu, M, K, N, group, True, gpu.bfloat16, M + N, True)
+    if K > 4104:
+        x.clamp_(-1, 1)
+    a = x.double() @ dense_on_device(gpu, *g, group)
+    wg = llk.Q4Weights.from_codes(*g, group=group)
+    if sides == 1:
+        assert gpu.equal(llk.q4_matmul(x, wg).double(), a)
+        acc = gpu.full((M, N), 0.5, dtype=gpu.float32, device="cuda")
+        assert gpu.equal(llk.q4_matmul(x, wg, out=acc, accumulate=True).double(), a + 0.5)
+        return
+    _, *u = case(gpu, M, K, N, group, False, gpu.float16, M + N + 1, True)
+    b = x.double() @ dense_on_device(gpu, *u, group)
+    wu = llk.Q4Weights.from_codes(*u, group=group)
+    want = a / (1 + gpu.exp(-a)) * b
+    # the activation's 4 ulp, of its exponent's argument two roundings of |a| 2^-24, and
+    # its product
+    near = (a.abs() + 8) * 2.0 ** -23 * want.abs() + 1e-30
+    got = llk.q4_swiglu(x, wg, wu, out_dtype=gpu.float32).double()
+    assert ((got - want).abs() <= near).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(14, 5120, 12872), (15, 4096, 12840)])
+def test_a_captured_swiglu_against_its_sums(llk, gpu, M, K, N):
+    """More than 64 KiB of LDS, captured and replayed, against 64 bits."""
+    x, *g = case(gpu, M, K, N, 64, True, gpu.float16, 9, True)
+    _, *u = case(gpu, M, K, N, 64, True, gpu.float16, 10, True)
+    x.clamp_(-1, 1)
+    dense_g, dense_u = (dense_on_device(gpu, *s, 64) for s in (g, u))
+    wg, wu = (llk.Q4Weights.from_codes(*s, group=64) for s in (g, u))
+    side = gpu.cuda.Stream()
+    gpu.cuda.synchronize()
+    graph = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(graph, stream=side):
+        out = llk.q4_swiglu(x, wg, wu, out_dtype=gpu.float32)
+    for n in range(3):
+        x.copy_(x.roll(n, 1))
+        graph.replay()
+        a, b = x.double() @ dense_g, x.double() @ dense_u
+        want = a / (1 + gpu.exp(-a)) * b
+        near = (a.abs() + 8) * 2.0 ** -23 * want.abs() + 1e-30
+        assert ((out.double() - want).abs() <= near).all()
