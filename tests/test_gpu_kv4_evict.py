@@ -296,3 +296,53 @@ def test_new_lengths_in_a_shifted_view(llk, gpu):
     new, source = llk.kv4_evict_plan(w, table, six[:3], 25, lens_out=six[3:])
     assert new.tolist() == [25, 25, 20] and six[:3].tolist() == [40, 30, 20]
     assert gpu.equal(source, llk.kv4_evict_plan(w, table, lens, 25)[1])
+
+
+def test_a_stream_of_the_callers(llk, gpu):
+    """Plan and move on another stream, which is behind, while the current one goes on;
+    a captured step whose two calls are given the capturing stream."""
+    D, size, keep = 64, 16, 50
+    p = Pool(gpu, [120, 49, 90], 2, size, 14)
+    w, pos, table, lens = p.dev()
+    data = p.rng.integers(0, 256, (w.shape[0], 2, 17 * D)).astype(np.uint8)
+    cache = gpu.from_numpy(data.copy()).cuda()
+    want_len, want = plan(p.weights, p.positions, p.table, p.lens, keep, 9, 2)
+    want_cache, (want_w, want_pos) = moved(data, p.table, want, keep, size, D, [p.weights, p.positions])
+    big = [gpu.zeros(1 << 28, dtype=gpu.uint8, device="cuda") for _ in range(2)]
+    side = gpu.cuda.Stream()
+    held = [t.clone() for t in (cache, w, pos, lens)]
+    new = gpu.full_like(lens, -1)
+
+    def step():
+        _, source = llk.kv4_evict_plan(w, table, lens, keep, positions=pos, recent=9, first=2,
+                                       lens_out=new, stream=side)
+        llk.kv4_evict(cache, table, source, head_dim=D, weights=w, positions=pos, lens=lens, stream=side)
+        return source
+
+    def check(source):
+        assert np.array_equal(source.cpu().numpy(), want)
+        assert np.array_equal(new.cpu().numpy(), want_len) and gpu.equal(new, lens)
+        for got, expect in ((cache, want_cache), (w, want_w), (pos, want_pos)):
+            assert np.array_equal(got.cpu().numpy(), expect)
+
+    gpu.cuda.synchronize()
+    with gpu.cuda.stream(side):
+        for n in range(100):  # about 10 ms of copies
+            big[n % 2].copy_(big[1 - n % 2])
+        copied = gpu.cuda.Event()
+        copied.record()
+    source = step()
+    same = bool((new == -1).all())
+    if not copied.query():  # nothing of it ran on the current stream
+        assert same
+    gpu.cuda.synchronize()
+    check(source)
+    graph = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(graph, stream=side):
+        source = step()
+    for _ in range(3):
+        for t, was in zip((cache, w, pos, lens), held):
+            t.copy_(was)
+        new.fill_(-1)
+        graph.replay()
+        check(source)

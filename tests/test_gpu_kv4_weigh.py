@@ -283,3 +283,24 @@ def test_weights_beyond_32_bits(llk, gpu):
         _, source = llk.kv4_evict_plan(w, table, lens, 17)
         llk.kv4_evict(x, table, source, head_dim=D, weights=w)
     assert gpu.equal(pool, far) and gpu.equal(near, marks)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (20, 0), (33, 4), (256, 40)])
+def test_scores_that_a_window_leaves_unwritten(llk, gpu, window, sinks):
+    """A workspace of NaN: what the attention did not write of it has no part in the
+    weights, or in the result."""
+    D, group = 64, 4
+    c = Case(gpu, [1, 700, 1500, 33], [1, 1, 1, 1], 2, D, 16, seed=window)
+    q = _dev(gpu, c.queries(2 * group), gpu.bfloat16)
+    pool, table, lens, _ = c.dev()
+    kw = dict(window=window, sinks=sinks, max_len=1500)
+    need = llk.describe_kv4_attention(q, pool, table, lens, weigh=True, **kw)["workspace_bytes"]
+    got = []
+    for fill in (0xff, 0x00):
+        scratch = gpu.full((need,), fill, dtype=gpu.uint8, device="cuda")
+        weights = gpu.zeros(pool.shape[0], 2, 16, device="cuda")
+        out = llk.kv4_attention(q, pool, table, lens, weights=weights, scratch=scratch, **kw)
+        got.append((out, weights))
+    assert gpu.equal(got[0][0], got[1][0]) and gpu.equal(got[0][1], got[1][1])
+    assert got[0][1].isfinite().all()
+    run(llk, c, c.queries(2 * group), 0.5, window=window, sinks=sinks, max_len=1500)
