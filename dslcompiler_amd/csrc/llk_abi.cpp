@@ -105,7 +105,10 @@ int fail_hip(hipError_t e, const char* what) {
 
 constexpr int kMaxDevices = 64;
 
-// A library-owned workspace: device memory, zero-filled when allocated.
+// A library-owned workspace: device memory, not cleared.  A call reads nothing of it that
+// it did not write, or makes no use of it; and a fill of fresh device memory is work of the
+// null stream that hipMemset does not wait for, which would run among the calls of
+// the workspace's own stream whenever the null stream got to it.
 struct Workspace {
   void* ptr = nullptr;
   size_t bytes = 0;
@@ -309,11 +312,6 @@ int get_workspace(int dev, size_t need, size_t asked, llk_kernel_context* ctx, v
     if (e != hipSuccess)
       return fail(LLK_ERR_OUT_OF_MEMORY, "hipMalloc(%zu) for workspace: %s", bytes,
                   hipGetErrorString(e));
-    e = hipMemset(fresh, 0, bytes);
-    if (e != hipSuccess) {
-      (void)hipFree(fresh);
-      return fail_hip(e, "hipMemset(workspace)");
-    }
     w->ptr = fresh;
     w->bytes = bytes;
     w->pinned = false;
