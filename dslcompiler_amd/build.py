@@ -32,7 +32,7 @@ CXX = os.environ.get("CXX_HOST", "g++")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 # Packed-FP32 VALU forms (v_pk_*_f32) are disabled for all device code: some
-# of their forms have given wrong results on MI355X machines of this pool.
+# of their forms have given wrong results on MI355X machines.
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,7 +1,8 @@
 // decoder_ops.cpp -- C entry points of the operators around the MLP in a
-// decoder block (include/llk/llk_abi.h): the fused residual norm and the 4-bit
-// paged cache with the attention that reads it.  Kernels: kernels/block_norm.hip,
-// kernels/kv4_cache.hip, kernels/kv4_attention.hip.
+// decoder block (include/llk/llk_abi.h): the fused residual norm, the 4-bit paged cache
+// with the attention that reads it, the weights that it gave, and eviction by them.
+// Kernels: kernels/block_norm.hip, kernels/kv4_cache.hip, kernels/kv4_attention.hip,
+// kernels/kv4_prompt.hip, kernels/kv4_weigh.hip, kernels/kv4_evict.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -286,8 +287,8 @@ int check_attention(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk
 
 // The workspace of an attention that adds its weights up: the splits' parts, the rows'
 // statistics, and the scores of single tokens' rows.
-// (Bytes of scores: beyond it they are computed again, which takes 64 sequences to 8192
-// keys, 32 query heads on 8, from 108 us to 156.)
+// (Bytes of scores: beyond it they are computed again, as with `starts`: 64 sequences to
+// 8192 keys, 32 query heads on 8, 126 us a call in a replayed graph for 95.)
 constexpr int64_t kMaxKept = (int64_t)512 << 20;
 struct WeighPlan {
   size_t stats, kept, bytes;  // where they begin; all

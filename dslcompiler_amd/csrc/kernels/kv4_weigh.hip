@@ -7,12 +7,15 @@
 // one wave that goes over all its rows, so nothing is added from two places and the
 // sums come out the same every time.
 //
-// Single tokens (few rows): the attention stores its scores, 4 bytes for a row and key
-// where the cache has 17/16 D, and they are read once more here.  Where it did not,
-// or rows are many, the scores are computed again: a prompt has far more pairs of a
-// row and a key than could be kept.  64 ragged sequences to 8192 keys, 32 query heads
-// on 8: the attention 84 us with its scores stored (68 without) and 15 here, a call
-// 108 in all, and 156 with the scores computed again.
+// Single tokens without `starts`, to 16 query heads of a key head: the attention
+// stores its scores, 4 bytes for a row and key where the cache has 17/16 D, and they are
+// read once more here (also those of keys outside a window, which are not used).  Where
+// it did not, the scores are computed again: a prompt has far more pairs of a row and a
+// key than could be kept, and the buffer goes by sequence, of which a batch with
+// `starts` may have some with more tokens than one.  64 ragged sequences to 8192 keys, 32 query heads on 8: the
+// attention 84 us with its scores stored (68 without) and 15 here (kernel times).  A call
+// in a replayed graph, 4337 keys on average: 66 without weights, 95 with, 126 by
+// `starts`; with a window of 256 10, 24 and 65.
 #include <algorithm>
 #include <type_traits>
 
@@ -188,10 +191,13 @@ __global__ void __launch_bounds__(kWaves * 64)
 // half of them for either four.  S^T = K Q^T on v_mfma_f32_32x32x16_bf16, any order of
 // the D values: of a key's, the lane's half of the wave has the first or second half.
 //
-// What bounds it is LDS: every operand that is read meets one product.  A prompt of
-// 2048 tokens, 32 heads, takes 43 us (400 TFLOP/s of what causality leaves), 44
-// without the products or without the exponentials, and 38 with rows that stay in
-// LDS.  64 keys to a wave need more registers than there are (61 us).
+// A prompt of 2048 tokens, 32 heads, takes 41 us (400 TFLOP/s of what causality
+// leaves).  No unit is near its limit: vector instructions take 39% of a SIMD's
+// cycles, products 20%, LDS 22% of a CU's, without bank conflicts; taking out the
+// products or the exponentials changed nothing, keeping the rows in LDS a tenth.  At D =
+// 128 it has 193 registers, so eight waves to a CU, all in step by a barrier a round, and
+// they wait for 36% of their time.  A round's scores carried over to the next round's
+// products gained nothing; 64 keys to a wave need more registers than there are (61 us).
 constexpr int kRowWaves = 8, kRowThreads = kRowWaves * 64, kRowKeys = 128;
 
 template <int D>

@@ -17,8 +17,7 @@
 // the vector memory path, not HBM, would be the limit), and its 8 waves take the
 // range's units in turn, four of them on their way.  Their sums are joined in LDS, and
 // those of a split K by a second kernel.  SwiGLU of 4096 x 14336, 1 row: 12.3 us, 5.0
-// TB/s; 13824 x 5120, 5 rows: 11.4 us and 4.0 to join 6 splits.  With X from memory
-// 15.8 and 18.7.
+// TB/s; 13824 x 5120, 5 rows: 11.4 us and 4.0 to join 6 splits (kernel times).
 #include <algorithm>
 
 #include "common.h"
@@ -198,7 +197,9 @@ hipError_t launch_group(const Q4Args& a, const Q4Plan& p, hipStream_t s) {
 }  // namespace llk_gfx950
 
 // The kernel for 16 rows streams the weights once for them; the tile kernel shares
-// them among 32 or 64.
+// them among 32 or 64.  The figures are us a call in a replayed graph, the second
+// kernel of a split K included, on weights that come from HBM, groups of 128 where
+// nothing else is said.
 Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
   const int64_t units = std::max<int64_t>(1, q4_units(K));
   Q4Plan p{};
@@ -208,32 +209,40 @@ Q4Plan llk_plan_q4(int64_t M, int64_t N, int64_t K, int sides) {
   if (M <= 16 || K < 8) {  // (the tile kernel reads 8 elements of a row at once)
     // A workgroup's X takes 256 M bytes a unit of K.  Without a split of K a call is one
     // launch, about 3 us less than with the kernel that joins them; the columns are
-    // then a launch's only parallelism, so that few tiles go to a workgroup.  Measured,
-    // us, 1, 2 and 4 tiles: 4096 x 4096, 1 row, 4.7, 5.9, 8.4; 4096 x 14336, 9.6, 9.1,
-    // 9.5, SwiGLU 15.7, 15.1, 14.3.
+    // then a launch's only parallelism, so that few tiles go to a workgroup.  1, 2 and
+    // 4 tiles: 4096 x 4096, 1 row, 4.6, 5.6, 7.8; 4096 x 14336, 1 row, 9.1, 8.6, 8.8, 8
+    // rows 14.8, 11.4, 10.8; SwiGLU of it, 1 row, 14.7, 13.9, 13.1, 8 rows 20.3, 15.5,
+    // 15.0.  Near the limits the next choice may be a tenth faster: 4096 x 10240, 1 row,
+    // 7.5, 8.3, 8.5; SwiGLU of 4096 x 11008, 1 row, 12.1, 13.2, 12.0.
     p.rows = 16;
     const bool two = sides == 2;
     const int64_t x = std::min<int64_t>(M, 16) * units, four = (columns + 3) / 4;
     if (x <= 256 || (x <= 640 && two && four >= 200)) {
-      // (640 is all of a CU's LDS: SwiGLU of 5120 x 13824, 16 rows, 26.7 us, split by 2
-      // 32.6, by 3 35.8)
+      // (640 is all of a CU's LDS: SwiGLU of 5120 x 13824, 16 rows, 19.9, split by 2
+      // 23.1, by 3 26.0)
       p.tiles = two && columns >= 800 ? 4 : columns >= (two ? 400 : 640) ? 2 : 1;
       s = 1;
     } else {
       // Two workgroups to a CU, 4 tiles each, at least 8 units.  13824 x 5120, 5 rows: 1
-      // tile, 1 split 18.4, 2 tiles, 3 splits 15.3, 4 tiles, 6 splits 15.2; 16 rows 30.5,
-      // 21.1 and 17.2.  4096 x 4096, 16 rows: 2 tiles, 2 splits 9.4, 4 and 4 8.5.
+      // tile, 1 split 20.7, 2 tiles, 3 splits 14.6, 4 tiles, 6 splits 13.8; 16 rows, 3
+      // splits with 1, 2 and 4 tiles 32.6, 23.1, 18.0, 4 tiles, 6 splits 16.8.  4096 x
+      // 4096, 16 rows: 2 tiles, 2 splits 9.2, 4 and 4 8.3.
       p.tiles = 4;
       s = std::max((x + 319) / 320, std::min(480 / four, units / 8));
     }
   } else {
     // 64 rows read the codes half as often, 32 leave more workgroups that hide their
-    // waits.  Measured, us, 32 and 64: 4096 x 4096, 64 rows, 15.3, 18.7, 128 rows 21.8,
-    // 23.6; 13824 x 5120, 255 rows, 75.6, 68.6; SwiGLU of 4096 x 14336, 64 rows, 35.5, 35.1.
+    // waits.  32 and 64: 4096 x 4096, 64 rows, 15.0, 18.6, 128 rows 20.7, 23.0; 13824 x
+    // 5120, 128 rows, 36.0, 36.8, 255 rows 59.7, 56.1, 512 rows 145, 98; groups of 32,
+    // 128 rows, 49.1, 50.6 (with 8 registers spilled), 255 rows 86, 82, groups of 64 41.1,
+    // 40.0, 69, 62; SwiGLU of 4096 x 14336, 64 rows, 32.3, 33.6, 255 rows 87, 75.  Between
+    // 129 and 192 rows it goes by how many workgroups there are: 129 rows, 4096 x 4096,
+    // 21.8, 26.4; 13824 x 5120 40.2, 44.1; 5120 x 13824 57.7, 47.5.
     p.rows = M <= 128 ? 32 : 64;
     const int64_t tiles = (M + p.rows - 1) / p.rows * ((N * sides + 255) / 256);
     // Two workgroups to a CU, at least 4 units to each.  SwiGLU of 4096 x 14336, 32 rows:
-    // 512 workgroups 23.5 us, 768 26.3, 1024 28.0; 13824 x 5120, 17 rows, 18.8, 20.6, 20.6.
+    // 448 workgroups 21.7, 672 25.3, 896 27.0; 13824 x 5120, 17 rows, 440 17.6, 540 20.3,
+    // 720 19.0.
     s = std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, units / 4));
   }
   p.stages = (int)((units + s - 1) / s);

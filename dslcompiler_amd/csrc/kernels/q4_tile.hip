@@ -7,11 +7,12 @@
 // sums of each row over a group, which the threads that move X add up on the way.
 //
 // What bounds it from 64 rows on are the vector and the matrix instructions, which
-// take turns: 13824 x 5120, 255 rows, 52 us (700 TFLOP/s), vector 47% and matrix 36% of
-// a SIMD's cycles; a column tile's sums and the next one's conversions between the
-// products of one, in a given order, measured 8% more.  SwiGLU of 5120 x 13824, 17
-// rows, groups of 32, 26 us: the scales and zeros of 32 rows each 32 k; codes two units
-// ahead measured 4% more.
+// take turns: 13824 x 5120, 255 rows, 52 us (700 TFLOP/s; the kernel without the one
+// that joins its splits, 9), vector 47% and matrix 36% of a SIMD's cycles; a column
+// tile's sums and the next one's conversions between the products of one, in a given
+// order, measured 8% more.  SwiGLU of 5120 x 13824, 17 rows, groups of 32, 26 us (and 5
+// to join): the scales and zeros of 32 rows each 32 k; codes two units ahead measured 4%
+// more.
 #include <algorithm>
 
 #include "common.h"

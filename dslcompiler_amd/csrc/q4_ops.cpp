@@ -1,5 +1,6 @@
 // q4_ops.cpp -- C entry points of the weights in 4 bits (include/llk/llk_abi.h).
-// Kernels: kernels/q4_pack.hip, kernels/q4_gemv.hip.
+// Kernels: kernels/q4_pack.hip, kernels/q4_gemv.hip (few rows; the plan of both),
+// kernels/q4_tile.hip.
 #include <hip/hip_runtime.h>
 
 #include <cstdarg>
