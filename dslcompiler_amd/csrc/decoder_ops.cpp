@@ -340,6 +340,9 @@ int attend(const llk_tensor3d* q, const llk_kv4_cache* cache, const llk_kv4_batc
       return fail(LLK_ERR_INVALID_ARGUMENT, "decay %g is negative or not finite", decay);
   }
   if (empty) return LLK_OK;
+  // (the scores that are not kept are computed from q once more)
+  if (marks && out->data == q->data)
+    return fail(LLK_ERR_INVALID_ARGUMENT, "with weights out must not be q");
   a.out = bf16_of(out);
   a.out_token = out->stride0;
   a.out_head = out->stride1;

@@ -299,7 +299,8 @@ def kv4_attention(q, cache, table, lens, *, starts=None, scale: float | None = N
     weights (of :func:`kv4_marks`): in every slot of a sequence with new tokens,
     decay times what was there (with 0 it is not read) plus the softmax weights
     that the new tokens' query heads gave it.  A page that is in the table twice
-    (a prefix that two sequences share) gets sums without order."""
+    (a prefix that two sequences share) gets sums without order.  out must not be
+    q then."""
     dev = _begin()
     args = _attention(q, cache, table, lens, starts, scale, window, sinks, max_len, dev)
     if out is None:

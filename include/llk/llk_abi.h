@@ -435,7 +435,7 @@ int llk_kv4_write_marked(const llk_tensor3d* k, const llk_tensor3d* v, const llk
  * no page is in the tables twice (two sequences that share one add up without order).
  * Other slots are left as they are.  A row without a key it sees adds nothing, one
  * that is NaN makes the slots that it sees NaN.  The result is that of
- * llk_kv4_attention, bit for bit. */
+ * llk_kv4_attention, bit for bit; out must not overlap q, which is read after it. */
 int llk_kv4_attention_weigh(const llk_tensor3d* q, const llk_kv4_cache* cache,
                             const llk_kv4_batch* batch, const llk_attention_params* params,
                             const llk_kv4_marks* marks, float decay, llk_tensor3d* out,

@@ -78,6 +78,18 @@ def test_attention_refusals(L):
                                      e, None) == 0
 
 
+def test_a_result_over_the_queries(L):
+    """The weights are computed from q once more, after the result is there."""
+    q = _kv(H=8)
+
+    def call(out, **b):
+        return L.llk_kv4_attention_weigh(q, _cache(), _batch(**b), _par(), _marks(), 1.0, out, None)
+
+    assert call(q) == -1 and b"out" in L.llk_last_error()
+    assert call(_kv(H=8, s0=4096)) == -1  # the same memory at other strides
+    assert call(_kv(H=8, data=2 * FAKE)) != -1  # (no device here)
+
+
 def test_attention_plans(L):
     """The rows' statistics, and of single tokens the scores up to 512 MiB, come on
     top of the attention's own workspace."""
